@@ -23,7 +23,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJDIR = os.path.join(ROOT, "_build")
 LIB = os.path.join(HERE, "libflower_amd.so")
 DIAG_LIB = os.path.join(HERE, "libflower_amd_diag.so")
-SOURCES = ["flw_error.hip", "flw_quant.hip", "flw_swa.hip", "flw_swa_bf16.hip", "flw_gemm.hip", "flw_heads.hip", "flw_norm_act.hip"]
+SOURCES = ["flw_error.hip", "flw_quant.hip", "flw_swa.hip", "flw_swa_bf16.hip", "flw_gemm.hip", "flw_heads.hip", "flw_norm_act.hip",
+           "flw_rope.hip", "flw_paged.hip", "flw_pages.hip"]
 # The diagnostics library: its own source plus its own copy of the error / timing state.
 DIAG_SOURCES = ["diag/flw_diag.hip"]
 NATIVE = os.path.join(HERE, "_native.so")
@@ -44,7 +45,7 @@ COMMON = [
 # sizes; the other head dims compile alike). The other sources keep the compiler's default forms.
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 PER_SOURCE = {"flw_swa.hip": [*VGPR_FORM, "-fno-honor-nans", "-mno-amdgpu-ieee"], "flw_gemm.hip": VGPR_FORM,
-              "flw_swa_bf16.hip": VGPR_FORM}
+              "flw_swa_bf16.hip": VGPR_FORM, "flw_paged.hip": VGPR_FORM}
 NOISE = "'-packed-fp32-ops' is not a recognized feature"
 
 

@@ -15,10 +15,11 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libflower_amd.so")
 
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
 SCALE_TENSOR, SCALE_HEAD, SCALE_BH, SCALE_COLUMN = 0, 1, 2, 3
 LAYOUT_BHTD, LAYOUT_VTILE, LAYOUT_BTHD = 0, 1, 2
 GEMM_A8W8, GEMM_W8A16 = 0, 1
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 
 GRANULARITY = {"tensor": SCALE_TENSOR, "head": SCALE_HEAD, "bh": SCALE_BH}
 
@@ -124,6 +125,30 @@ SIGNATURES = {
     "flw_swa_bf16_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                  c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                  c_void_p]),
+    "flw_rope": (c_int, [c_void_p, _P64, c_int64, c_void_p, _P64, c_int64, c_int, c_int64, c_int64, c_int64, c_void_p,
+                         c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p,
+                         c_void_p]),
+    "flw_paged_append": (c_int, [c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_int64, c_int64, c_int64, c_int64,
+                                 c_int64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                 c_void_p, c_int, c_float, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_void_p]),
+    "flw_paged_attention_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                                       c_int64]),
+    "flw_paged_attention": (c_int, [c_void_p, _P64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                    c_int64, c_int64, c_float, c_void_p, _P64, c_void_p, c_void_p, c_size_t,
+                                    c_void_p]),
+    "flw_reserve_pages_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "flw_reserve_pages": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "flw_reorder_pages_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "flw_reorder_pages": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                  c_void_p, c_size_t, c_void_p]),
+    "flw_compact_pages_workspace_bytes": (c_size_t, [c_int64]),
+    "flw_compact_pages": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                  c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                  c_void_p]),
     "flw_fp8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
     "flw_fp8_linear": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                c_int64, c_int, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),

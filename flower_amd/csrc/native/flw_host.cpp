@@ -5,6 +5,7 @@
 // its autograd node and its module stay in Python: nothing here records a graph, and every function
 // takes the stream it launches on (torch's current stream of the tensors' device, as a handle).
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -387,6 +388,123 @@ std::tuple<Tensor, Tensor> qkv_norm_rope_amax(const Tensor& a8, const Tensor& sa
   return {y, amax};
 }
 
+// ---------------------------------------------------------------- rotary positions, paged cache
+// These run on the device of their tensors, whichever is current.
+
+int32_t* i32(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+int32_t* i32(const OptTensor& t) { return t ? i32(*t) : nullptr; }
+float* f32(const OptTensor& t) { return t ? f32(*t) : nullptr; }
+int cache_code(const Tensor& pages) { return pages.scalar_type() == at::kBFloat16 ? FLW_BF16 : FLW_E4M3; }
+
+// in_place, where a dimension of one has whatever stride.
+Tensor heads(const Tensor& x, int64_t* st) {
+  const int64_t vec = x.scalar_type() == at::kFloat ? 4 : 8;
+  bool ok = x.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (x.size(i) == 1 || x.stride(i) % vec == 0);
+  Tensor y = ok ? x : x.clone(at::MemoryFormat::Contiguous);
+  for (int i = 0; i < 3; ++i) st[i] = y.size(i) == 1 ? 0 : y.stride(i);
+  return y;
+}
+
+std::tuple<Tensor, OptTensor> rope(const Tensor& q0, const OptTensor& k0, const Tensor& cos, const Tensor& sin,
+                                   const OptTensor& positions, bool half, bool inverse, int64_t stream) {
+  c10::DeviceGuard guard(q0.device());
+  int64_t st[6] = {};
+  Tensor q = heads(q0, st), qo = empty(q0, q0.sizes(), q0.scalar_type());
+  OptTensor k, ko;
+  if (k0) {
+    k = heads(*k0, st + 3);
+    ko = empty(*k0, k0->sizes(), k0->scalar_type());
+  }
+  const int bits = positions && positions->scalar_type() == at::kLong ? 64 : 32;
+  check(flw_rope(q.data_ptr(), st, q.size(1), opt(k), st + 3, k ? k->size(1) : 0, dtype_code(q), q.size(0), q.size(2), q.size(3),
+                 f32(cos), f32(sin), cos.size(0), 2 * cos.size(1), half ? FLW_ROPE_HALF : FLW_ROPE_INTERLEAVED, inverse,
+                 opt(positions), bits, positions && positions->dim() == 2 ? positions->stride(0) : 0, qo.data_ptr(), opt(ko),
+                 str(stream)),
+        "apply_rotary");
+  return {qo, ko};
+}
+
+std::tuple<Tensor, OptTensor> paged_append(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& k_pages,
+                                           const Tensor& v_pages, const Tensor& tables, const Tensor& lens,
+                                           const OptTensor& counts, const std::optional<double>& eps, const OptTensor& cos,
+                                           const OptTensor& sin, bool half, const OptTensor& k_scale,
+                                           const OptTensor& v_scale, bool return_k, int64_t stream) {
+  c10::DeviceGuard guard(q0.device());
+  int64_t st[9];
+  Tensor q = heads(q0, st), k = heads(k0, st + 3), v = heads(v0, st + 6);
+  Tensor qo = empty(q, q.sizes(), at::kBFloat16);
+  OptTensor ko;
+  if (return_k) ko = empty(k, k.sizes(), at::kBFloat16);
+  check(flw_paged_append(q.data_ptr(), st, k.data_ptr(), st + 3, v.data_ptr(), st + 6, q.size(0), q.size(1), k.size(1), q.size(2),
+                         q.size(3), k_pages.data_ptr(), v_pages.data_ptr(), cache_code(k_pages), k_pages.size(0),
+                         k_pages.size(2), i32(tables), tables.size(1), i32(lens), i32(counts), eps.has_value(),
+                         (float)eps.value_or(0.0), f32(cos), f32(sin), cos ? cos->size(0) : 0, cos ? 2 * cos->size(1) : 0,
+                         half ? FLW_ROPE_HALF : FLW_ROPE_INTERLEAVED, f32(k_scale), f32(v_scale), qo.data_ptr(), opt(ko),
+                         str(stream)),
+        "paged_append");
+  return {qo, ko};
+}
+
+// out (B, H, T, D), a view of token-major storage, and the log-sum-exp when asked for.
+std::tuple<Tensor, OptTensor> paged_attention(const Tensor& q0, const Tensor& k_pages, const Tensor& v_pages,
+                                              const Tensor& tables, const Tensor& lens, const OptTensor& counts,
+                                              int64_t window, double scale, const OptTensor& k_scale,
+                                              const OptTensor& v_scale, bool with_lse, int64_t stream) {
+  c10::DeviceGuard guard(q0.device());
+  int64_t st[6];
+  Tensor q = heads(q0, st);
+  const int64_t B = q.size(0), H = q.size(1), T = q.size(2), D = q.size(3), KV = k_pages.size(1), page = k_pages.size(2);
+  Tensor out = empty(q, {B, T, H, D}, at::kBFloat16);
+  st[3] = T * H * D; st[4] = D; st[5] = H * D;
+  OptTensor lse, ws;
+  if (with_lse) lse = empty(q, {B, H, T}, at::kFloat);
+  const size_t need = flw_paged_attention_workspace_bytes(B, H, KV, T, D, page, tables.size(1), window);
+  if (need > 0) ws = workspace(q, need);
+  check(flw_paged_attention(q.data_ptr(), st, k_pages.data_ptr(), v_pages.data_ptr(), cache_code(k_pages), k_pages.size(0), page,
+                            i32(tables), tables.size(1), i32(lens), i32(counts), f32(k_scale), f32(v_scale), B, H, KV, T, D,
+                            window, (float)scale, out.data_ptr(), st + 3, f32(lse), opt(ws), need, str(stream)),
+        "paged_attention");
+  return {out.transpose(1, 2), lse};
+}
+
+Tensor reserve_pages(const Tensor& tables, const Tensor& lens, const Tensor& refs, const Tensor& counts, int64_t page,
+                     int64_t window, const Tensor& tables_out, const Tensor& lens_out, const Tensor& refs_out,
+                     int64_t stream) {
+  c10::DeviceGuard guard(tables.device());
+  const int64_t S = tables.size(0), P = refs.size(0);
+  Tensor granted = empty(lens, {S}, at::kInt), ws = workspace(lens, flw_reserve_pages_workspace_bytes(S, P));
+  check(flw_reserve_pages(i32(tables), i32(lens), i32(refs), i32(counts), S, tables.size(1), P, page, window, i32(tables_out),
+                          i32(lens_out), i32(refs_out), i32(granted), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
+        "reserve_pages");
+  return granted;
+}
+
+// k_pages, v_pages (L, P, KV, ..) as the two below take them.
+void reorder_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& lens, const Tensor& refs,
+                   const Tensor& parents, const Tensor& tables_out, const Tensor& lens_out, const Tensor& refs_out,
+                   int64_t stream) {
+  c10::DeviceGuard guard(tables.device());
+  const int64_t S = tables.size(0), M = tables.size(1), P = refs.size(0);
+  Tensor ws = workspace(lens, flw_reorder_pages_workspace_bytes(S, M, P));
+  check(flw_reorder_pages(k_pages.data_ptr(), v_pages.data_ptr(), cache_code(k_pages), k_pages.size(0), P, k_pages.size(2),
+                          k_pages.size(3), k_pages.size(4), i32(tables), i32(lens), i32(refs), i32(parents), S, M,
+                          i32(tables_out), i32(lens_out), i32(refs_out), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
+        "reorder_pages");
+}
+
+Tensor compact_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& refs,
+                     const Tensor& tables_out, const Tensor& refs_out, int64_t stream) {
+  c10::DeviceGuard guard(tables.device());
+  const int64_t P = refs.size(0);
+  Tensor live = empty(refs, {1}, at::kInt), ws = workspace(refs, flw_compact_pages_workspace_bytes(P));
+  check(flw_compact_pages(k_pages.data_ptr(), v_pages.data_ptr(), cache_code(k_pages), k_pages.size(0), P, k_pages.size(2),
+                          k_pages.size(3), k_pages.size(4), i32(tables), i32(refs), tables.size(0), tables.size(1),
+                          i32(tables_out), i32(refs_out), i32(live), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
+        "compact_pages");
+  return live;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -422,4 +540,10 @@ PYBIND11_MODULE(_native, m) {
   m.def("swiglu_bwd", &swiglu_bwd, nogil());
   m.def("act_quant_rows", &act_quant_rows, nogil());
   m.def("qkv_norm_rope_amax", &qkv_norm_rope_amax, nogil());
+  m.def("rope", &rope, nogil());
+  m.def("paged_append", &paged_append, nogil());
+  m.def("paged_attention", &paged_attention, nogil());
+  m.def("reserve_pages", &reserve_pages, nogil());
+  m.def("reorder_pages", &reorder_pages, nogil());
+  m.def("compact_pages", &compact_pages, nogil());
 }

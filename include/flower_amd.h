@@ -29,7 +29,8 @@ enum flw_status {
   FLW_E_LAUNCH = 4        /* HIP launch error */
 };
 
-enum flw_dtype { FLW_F32 = 0, FLW_BF16 = 1 };
+/* FLW_E4M3: what a paged key-value cache may hold besides bf16; the other entry points take e4m3 as codes. */
+enum flw_dtype { FLW_F32 = 0, FLW_BF16 = 1, FLW_E4M3 = 2 };
 
 /* Scale granularity for a (B, H, T, D) tensor: one scale, one per head h (amax over B, T, D),
  * or one per (b, h) slice (amax over T, D). Scale arrays hold 1, H or B*H floats. */
@@ -49,6 +50,9 @@ enum flw_layout { FLW_LAYOUT_BHTD = 0, FLW_LAYOUT_VTILE = 1, FLW_LAYOUT_BTHD = 2
 /* GEMM modes. A8W8: activations quantised per row to e4m3, FP8 x FP8 MFMA (the _fp8_head
  * recipe). W8A16: e4m3 weights widened to bf16 in the kernel, bf16 activations unquantised. */
 enum flw_gemm_mode { FLW_GEMM_A8W8 = 0, FLW_GEMM_W8A16 = 1 };
+
+/* Which values of a head a rotary pair is: 2 i and 2 i + 1, or i and i + rotary_dim / 2. */
+enum flw_rope_layout { FLW_ROPE_INTERLEAVED = 0, FLW_ROPE_HALF = 1 };
 
 const char* flw_last_error(void);
 int flw_abi_version(void);
@@ -444,6 +448,90 @@ int flw_swa_bf16_bwd_layout(const void* q, const void* k, const void* v, const v
                             int o_layout, const float* lse, int64_t B, int64_t H, int64_t T, int64_t D,
                             int64_t window, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/* ---------------------------------------------------------------- rotary positions */
+
+/* Rotary positions of q and k, forward (inverse = 0) or its gradient (inverse = 1: the angles negated). No counterpart of
+ * its own in the reference, whose RotaryEmbedding (flower/models/base.py:436-483) turns whole interleaved heads at
+ * positions 0 .. T - 1: the pairs of a head's first rotary_dim values, (a, b) -> (a c - b s, b c + a s), c / s = cos / sin
+ * [table_rows, rotary_dim / 2] fp32 at the token's position; layout: enum flw_rope_layout; the rest of the head copied.
+ * fp32 arithmetic, rounded once. q (B, H, T, D) and k (B, KV, T, D; NULL with KV = 0), fp32 or bf16, element strides
+ * {b, h, t}, 16-byte aligned rows; q_out / k_out contiguous. positions: NULL (token t at t), or int32 / int64
+ * (positions_bits) at b * positions_stride_b + t; a position outside the tables makes its pairs NaN. rotary_dim a multiple
+ * of 8 up to D; D in {32, 64, 128}. */
+int flw_rope(const void* q, const int64_t* q_strides, int64_t H, const void* k, const int64_t* k_strides, int64_t KV,
+             int dtype, int64_t B, int64_t T, int64_t D, const float* cos, const float* sin, int64_t table_rows,
+             int64_t rotary_dim, int layout, int inverse, const void* positions, int positions_bits,
+             int64_t positions_stride_b, void* q_out, void* k_out, void* stream);
+
+/* ---------------------------------------------------------------- paged key-value cache */
+
+/* A cache of S sequences (no counterpart in the reference, which has no incremental decoding). A layer's pool:
+ *   k_pages (num_pages, KV, page_size, D), v_pages (num_pages, KV, D, page_size), bf16 or e4m3 codes (cache_dtype) with one
+ *   fp32 scale a kv head (k_scale, v_scale: value = code * scale; NULL for bf16); V lies along the positions, as the
+ *   attention's product reads it. page_size: a power of two from 16 to 1024.
+ * tables (S, table_cols) int32: the page of positions [j page_size, (j + 1) page_size) of a sequence, -1 where it holds none;
+ * lens (S) int32: its positions; refs (num_pages) int32: the table entries that hold a page, 0 = free. A page that is not
+ * full belongs to one sequence. Where lens, counts or tables are wrong nothing outside the given buffers is touched: a
+ * token without a page is not written, a query that should see a key without a page, or stands past its table, is NaN.
+ *
+ * counts (S, may be NULL: T) int32: the new tokens of each sequence, the last ones of its lens: token t < counts[b] stands
+ * at position lens[b] - counts[b] + t; tokens t >= counts[b] are padding. */
+
+/* The new tokens' heads on their way into the cache: q and k normed over the head when qk_norm (x / sqrt(mean x^2 + eps),
+ * HeadRMSNorm, flower/models/base.py:341-357), turned by their positions when cos / sin are given (flw_rope's tables and
+ * layouts), k and v written to their pages (e4m3: rne(clamp(x / scale, +-448)), NaN kept). fp32 arithmetic, rounded once.
+ * q (B, H, T, D), k, v (B, KV, T, D) bf16, strides {b, h, t}, 16-byte aligned rows; q_out contiguous (B, H, T, D), zero for
+ * padding; k_out (contiguous (B, KV, T, D) bf16, the k that was written) may be NULL. */
+int flw_paged_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                     const int64_t* v_strides, int64_t B, int64_t H, int64_t KV, int64_t T, int64_t D, void* k_pages,
+                     void* v_pages, int cache_dtype, int64_t num_pages, int64_t page_size, const int32_t* tables,
+                     int64_t table_cols, const int32_t* lens, const int32_t* counts, int qk_norm, float eps,
+                     const float* cos, const float* sin, int64_t table_rows, int64_t rotary_dim, int layout,
+                     const float* k_scale, const float* v_scale, void* q_out, void* k_out, void* stream);
+
+/* Attention of the new tokens over their pages: out = softmax(scale q k^T) v over the keys j of the sequence with
+ * j <= i and i - j < window of the query at position i (window > 0; pass one no shorter than the table for full causal
+ * attention). Query head h reads kv head h / (H / KV). q, out (B, H, T, D) bf16, strides {b, h, t}, q rows 16-byte and out
+ * rows 8-byte aligned; lse (B, H, T) fp32 (natural log of the sum of exp(scores); may be NULL). A padding token, and a query
+ * without keys, gives zeros and an lse of -inf. fp32 softmax and sums. workspace: flw_paged_attention_workspace_bytes
+ * (parts of long sequences; 0 where none is cut). */
+size_t flw_paged_attention_workspace_bytes(int64_t B, int64_t H, int64_t KV, int64_t T, int64_t D, int64_t page_size,
+                                           int64_t table_cols, int64_t window);
+int flw_paged_attention(const void* q, const int64_t* q_strides, const void* k_pages, const void* v_pages, int cache_dtype,
+                        int64_t num_pages, int64_t page_size, const int32_t* tables, int64_t table_cols, const int32_t* lens,
+                        const int32_t* counts, const float* k_scale, const float* v_scale, int64_t B, int64_t H, int64_t KV,
+                        int64_t T, int64_t D, int64_t window, float scale, void* out, const int64_t* out_strides, float* lse,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Room for counts[s] new tokens of each sequence: entries wholly behind the window of its next token are given back when
+ * window > 0 (0: none), then the empty entries of the new positions are filled with free pages, the lowest numbers first, in
+ * the order of the sequences; lens_out = lens + counts and granted = counts. A sequence whose pages cannot be had (the sum of
+ * the wants up to it is more than there are free pages, or its table is too short) gets none: lens stays, granted is 0, as
+ * it is where counts[s] <= 0. The outputs may be the inputs (each as a whole). */
+size_t flw_reserve_pages_workspace_bytes(int64_t S, int64_t num_pages);
+int flw_reserve_pages(const int32_t* tables, const int32_t* lens, const int32_t* refs, const int32_t* counts, int64_t S,
+                      int64_t table_cols, int64_t num_pages, int64_t page_size, int64_t window, int32_t* tables_out,
+                      int32_t* lens_out, int32_t* refs_out, int32_t* granted, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* Place s becomes a copy of the sequence at parents[s] (itself: it stays; no place: it is emptied), for all s at once: fork,
+ * free, and a beam search's reordering. Full pages are shared; a last page that is not full stays with one child (the one in
+ * its parent's place, else the first), the others get a page of their own with its positions copied, in all L layers of the
+ * pools (L, num_pages, ...). A place whose page cannot be had is emptied (lens 0). The outputs may be the inputs. */
+size_t flw_reorder_pages_workspace_bytes(int64_t S, int64_t table_cols, int64_t num_pages);
+int flw_reorder_pages(void* k_pages, void* v_pages, int cache_dtype, int64_t L, int64_t num_pages, int64_t KV,
+                      int64_t page_size, int64_t D, const int32_t* tables, const int32_t* lens, const int32_t* refs,
+                      const int32_t* parents, int64_t S, int64_t table_cols, int32_t* tables_out, int32_t* lens_out,
+                      int32_t* refs_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The pages in use (refs not 0, live[0] of them) moved to the numbers below live[0], in all L layers: those of higher
+ * numbers, in ascending order, to the free numbers below, in ascending order. The outputs may be the inputs. */
+size_t flw_compact_pages_workspace_bytes(int64_t num_pages);
+int flw_compact_pages(void* k_pages, void* v_pages, int cache_dtype, int64_t L, int64_t num_pages, int64_t KV,
+                      int64_t page_size, int64_t D, const int32_t* tables, const int32_t* refs, int64_t S,
+                      int64_t table_cols, int32_t* tables_out, int32_t* refs_out, int32_t* live, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- GEMM */
 
