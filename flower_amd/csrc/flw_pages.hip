@@ -52,7 +52,7 @@ static void copy_ints(CopyInts c, hipStream_t s) {
     most = most > c.n[a] ? most : c.n[a];
   }
   if (most == 0) return;
-  int64_t blocks = (most + 1023) / 1024;
+  int64_t blocks = (most + 255) / 256;
   blocks = blocks > 1024 ? 1024 : blocks;
   (void)launch_args(reinterpret_cast<const void*>(&copy_ints_kernel), dim3((unsigned)blocks), dim3(256), 0, s, nullptr,
                     nullptr, c);
@@ -271,34 +271,49 @@ struct PageCopy {
   int L, KV, D, page, size;       // size: bytes a value
 };
 
-// Reorder: the first `used` positions of page src to page dst; one workgroup a (place, layer, kv head, k or v).
+// Reorder: the first `used` positions of page src to page dst; one workgroup a (place, layer, k or v, kCopyHeads heads). A
+// thread takes one 16-byte run of a head's page, of each of the heads: their loads are in flight together.
+constexpr int kCopyHeads = 4;
 __global__ __launch_bounds__(256) void copy_tail_kernel(PageCopy p) {
   const int s = blockIdx.x;
   const int32_t dst = p.pairs[3 * s], src = p.pairs[3 * s + 1];
   if (dst < 0) return;
   const int used = p.pairs[3 * s + 2];
-  const int of = (int)blockIdx.y >> 1, layer = of / p.KV, head = of - layer * p.KV;
+  const int groups = (p.KV + kCopyHeads - 1) / kCopyHeads;
+  const int of = (int)blockIdx.y >> 1, layer = of / groups, h0 = (of - layer * groups) * kCopyHeads;
+  const int nh = p.KV - h0 < kCopyHeads ? p.KV - h0 : kCopyHeads;
   const int64_t bytes = (int64_t)p.page * p.D * p.size;
   uint8_t* pool = blockIdx.y & 1 ? p.v : p.k;
-  const uint8_t* a = pool + (((int64_t)layer * p.P + src) * p.KV + head) * bytes;
-  uint8_t* b = pool + (((int64_t)layer * p.P + dst) * p.KV + head) * bytes;
-  if ((blockIdx.y & 1) == 0) {
-    const int n = used * p.D * p.size / 16;                  // D x size is a multiple of 32
-    for (int i = threadIdx.x; i < n; i += 256) reinterpret_cast<uint4*>(b)[i] = reinterpret_cast<const uint4*>(a)[i];
-    return;
-  }
-  // each row of `page` positions: whole 16-byte runs, then the values of the last one
-  const int per = p.page * p.size / 16, fill = used * p.size, mine = (fill + 15) / 16;
-  for (int i = threadIdx.x; i < p.D * mine; i += 256) {
-    const int row = i / mine, c = i - row * mine;
-    const int64_t at = ((int64_t)row * per + c) * 16;
-    if (16 * c + 16 <= fill) {
-      *reinterpret_cast<uint4*>(b + at) = *reinterpret_cast<const uint4*>(a + at);
-    } else {
-      for (int j = 16 * c; j < fill; j += p.size) {
-        if (p.size == 2) *reinterpret_cast<uint16_t*>(b + at + j - 16 * c) = *reinterpret_cast<const uint16_t*>(a + at + j - 16 * c);
-        else b[at + j - 16 * c] = a[at + j - 16 * c];
+  const uint8_t* a = pool + (((int64_t)layer * p.P + src) * p.KV + h0) * bytes;
+  uint8_t* b = pool + (((int64_t)layer * p.P + dst) * p.KV + h0) * bytes;
+  const bool rows = blockIdx.y & 1;
+  // k: `used` rows of D values, a whole number of runs. v: of each of D rows the first `used` values; `per` runs a row.
+  const int lper = __builtin_ctz((unsigned)(p.page * p.size / 16)), per = 1 << lper;
+  const int n = rows ? p.D << lper : used * p.D * p.size / 16, fill = used * p.size;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int left = rows ? fill - 16 * (i & (per - 1)) : 16;
+    if (left <= 0) continue;
+    uint4 x[kCopyHeads];
+#pragma unroll
+    for (int h = 0; h < kCopyHeads; ++h)
+      if (h < nh) x[h] = *reinterpret_cast<const uint4*>(a + h * bytes + 16 * (int64_t)i);
+#pragma unroll
+    for (int h = 0; h < kCopyHeads; ++h) {
+      if (h >= nh) continue;
+      uint4* to = reinterpret_cast<uint4*>(b + h * bytes + 16 * (int64_t)i);
+      if (left < 16) {                     // the row's last run: what lies behind `used` stays (its one writer is this thread)
+        const uint4 was = *to;
+        uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
+        const uint32_t o[4] = {was.x, was.y, was.z, was.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = left - 4 * e;                          // bytes of this word to take
+          const uint32_t m = k >= 4 ? 0xFFFFFFFFu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
+          w[e] = (w[e] & m) | (o[e] & ~m);
+        }
+        x[h] = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      *to = x[h];
     }
   }
 }
@@ -483,8 +498,8 @@ extern "C" int flw_reorder_pages(void* k_pages, void* v_pages, int cache_dtype, 
   const Timer tm = take_timer();
   (void)launch_ext(reinterpret_cast<const void*>(&reorder_rows_kernel), dim3((unsigned)S), dim3(256), 0, s, p, tm.start, nullptr);
   (void)launch_ext(reinterpret_cast<const void*>(&reorder_take_kernel), dim3(1), dim3(kScan), 0, s, p, nullptr, nullptr);
-  (void)launch_ext(reinterpret_cast<const void*>(&copy_tail_kernel), dim3((unsigned)S, (unsigned)(2 * L * KV)), dim3(256), 0, s,
-                   c, nullptr, tm.stop);
+  (void)launch_ext(reinterpret_cast<const void*>(&copy_tail_kernel), dim3((unsigned)S, (unsigned)(2 * L * ((KV + kCopyHeads - 1) / kCopyHeads))),
+                   dim3(256), 0, s, c, nullptr, tm.stop);
   return check_launch("flw_reorder_pages");
 }
 
