@@ -258,6 +258,11 @@ def stream_of(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+def stream_or_none(t: torch.Tensor) -> int:
+    """stream_of(t), 0 for a tensor off the GPU: for the native operators that refuse such a tensor themselves."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device()) if t.is_cuda else 0
+
+
 _native_mod = None
 
 

@@ -2,13 +2,19 @@
 // the C ABI. What bounds a small call is the host (a 16-token FP8 linear: two kernels of 2.6 and 4.3
 // us behind 21 us of Python), and in Python every allocation, stream look-up and ctypes call costs
 // 1.5 to 3 us; here an allocate-and-launch body is one call. The checks of an operator's arguments,
-// its autograd node and its module stay in Python: nothing here records a graph, and every function
-// takes the stream it launches on (torch's current stream of the tensors' device, as a handle).
+// its autograd node and its module stay in Python, and every function takes the stream it launches on
+// (torch's current stream of the tensors' device, as a handle). The rotary positions and the paged
+// cache's operators are here as a whole, their checks and the one's autograd node too: their kernels
+// take 3 to 6 us in a decode step, less than the same checks take in Python.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cmath>
 #include <optional>
+#include <sstream>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -389,7 +395,29 @@ std::tuple<Tensor, Tensor> qkv_norm_rope_amax(const Tensor& a8, const Tensor& sa
 }
 
 // ---------------------------------------------------------------- rotary positions, paged cache
-// These run on the device of their tensors, whichever is current.
+// These check their arguments here and run on the device of their tensors, whichever is current.
+
+template <typename... A>
+std::string text(const A&... a) {
+  std::ostringstream s;
+  (s << ... << a);
+  return s.str();
+}
+#define REFUSE_UNLESS(cond, ...) \
+  do {                           \
+    if (!(cond)) throw py::value_error(text(__VA_ARGS__)); \
+  } while (0)
+
+void require_gpu(const Tensor& t) {
+  if (!t.is_cuda())
+    throw std::runtime_error(text("flower_amd operators run only on a ROCm GPU (gfx950); got a tensor on ", t.device(),
+                                  ". There is no CPU fallback."));
+}
+void check_ints(const char* name, const Tensor& t, at::IntArrayRef sizes, const Tensor& with) {
+  REFUSE_UNLESS(t.scalar_type() == at::kInt && t.sizes() == sizes && t.is_contiguous() && t.device() == with.device(), name,
+                " must be a contiguous int32 tensor ", sizes, " on ", with.device(), ", got ", t.sizes(), " ", t.scalar_type(),
+                " on ", t.device());
+}
 
 int32_t* i32(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 int32_t* i32(const OptTensor& t) { return t ? i32(*t) : nullptr; }
@@ -406,30 +434,162 @@ Tensor heads(const Tensor& x, int64_t* st) {
   return y;
 }
 
-std::tuple<Tensor, OptTensor> rope(const Tensor& q0, const OptTensor& k0, const Tensor& cos, const Tensor& sin,
-                                   const OptTensor& positions, bool half, bool inverse, int64_t stream) {
+void check_head_dim(int64_t D) { REFUSE_UNLESS(D == 32 || D == 64 || D == 128, "head_dim must be 32/64/128, got ", D); }
+
+void check_rotary_tables(const Tensor& cos, const Tensor& sin, const Tensor& q) {
+  REFUSE_UNLESS(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat,
+                "cos and sin must be float32 [positions, rotary_dim / 2] tables of one shape, got ", cos.sizes(), " ",
+                cos.scalar_type(), " and ", sin.sizes(), " ", sin.scalar_type());
+  REFUSE_UNLESS(cos.size(0) > 0 && cos.is_contiguous() && sin.is_contiguous() && cos.data_ptr() != nullptr &&
+                    reinterpret_cast<uintptr_t>(cos.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(sin.data_ptr()) % 16 == 0,
+                "cos and sin must be contiguous, 16-byte aligned and not empty");
+  const int64_t R = 2 * cos.size(1);
+  REFUSE_UNLESS(R > 0 && R <= q.size(3) && R % 8 == 0, "rotary_dim must be a multiple of 8 up to the head_dim ", q.size(3),
+                ", got ", R);
+  REFUSE_UNLESS(cos.device() == q.device() && sin.device() == q.device(), "cos and sin must be on ", q.device());
+  REFUSE_UNLESS(!(c10::GradMode::is_enabled() && (cos.requires_grad() || sin.requires_grad())),
+                "the rotary tables take no gradient");
+}
+
+// q, k (undefined: none) turned, contiguous: (q') or (q', k').
+std::vector<Tensor> rope(const Tensor& q0, const Tensor& k0, const Tensor& cos, const Tensor& sin, const Tensor& positions,
+                         bool half, bool inverse, int64_t stream) {
   c10::DeviceGuard guard(q0.device());
   int64_t st[6] = {};
-  Tensor q = heads(q0, st), qo = empty(q0, q0.sizes(), q0.scalar_type());
-  OptTensor k, ko;
-  if (k0) {
-    k = heads(*k0, st + 3);
-    ko = empty(*k0, k0->sizes(), k0->scalar_type());
+  Tensor q = heads(q0, st), k;
+  std::vector<Tensor> out{empty(q0, q0.sizes(), q0.scalar_type())};
+  if (k0.defined()) {
+    k = heads(k0, st + 3);
+    out.push_back(empty(k0, k0.sizes(), k0.scalar_type()));
   }
-  const int bits = positions && positions->scalar_type() == at::kLong ? 64 : 32;
-  check(flw_rope(q.data_ptr(), st, q.size(1), opt(k), st + 3, k ? k->size(1) : 0, dtype_code(q), q.size(0), q.size(2), q.size(3),
-                 f32(cos), f32(sin), cos.size(0), 2 * cos.size(1), half ? FLW_ROPE_HALF : FLW_ROPE_INTERLEAVED, inverse,
-                 opt(positions), bits, positions && positions->dim() == 2 ? positions->stride(0) : 0, qo.data_ptr(), opt(ko),
-                 str(stream)),
+  const bool pos = positions.defined();
+  check(flw_rope(q.data_ptr(), st, q.size(1), k.defined() ? k.data_ptr() : nullptr, st + 3, k.defined() ? k.size(1) : 0,
+                 dtype_code(q), q.size(0), q.size(2), q.size(3), f32(cos), f32(sin), cos.size(0), 2 * cos.size(1),
+                 half ? FLW_ROPE_HALF : FLW_ROPE_INTERLEAVED, inverse, pos ? positions.data_ptr() : nullptr,
+                 pos && positions.scalar_type() == at::kLong ? 64 : 32, pos && positions.dim() == 2 ? positions.stride(0) : 0,
+                 out[0].data_ptr(), k.defined() ? out[1].data_ptr() : nullptr, str(stream)),
         "apply_rotary");
-  return {qo, ko};
+  return out;
+}
+
+// The rotation is linear, its gradient the opposite rotation of the gradient: the node is its own backward. The backward runs
+// on the stream that the forward ran on, as torch's engine runs it.
+struct RopeNode : torch::autograd::Function<RopeNode> {
+  static std::vector<Tensor> forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k,
+                                     const Tensor& cos, const Tensor& sin, const OptTensor& positions, bool half, bool inverse,
+                                     int64_t stream) {
+    const Tensor pos = positions.value_or(Tensor());
+    ctx->save_for_backward({cos, sin, pos});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["how"] = (int64_t)(half | inverse << 1 | k.has_value() << 2);
+    ctx->saved_data["stream"] = stream;
+    return rope(q, k.value_or(Tensor()), cos, sin, pos, half, inverse, stream);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    torch::autograd::variable_list out(8);
+    const auto saved = ctx->get_saved_variables();
+    const int64_t how = ctx->saved_data["how"].toInt(), stream = ctx->saved_data["stream"].toInt();
+    const bool two = how & 4, q = g[0].defined(), k = two && g[1].defined();
+    if (!q && !k) return out;
+    const auto x = apply(q ? g[0] : g[1], q && k ? OptTensor(g[1]) : OptTensor(), saved[0], saved[1],
+                         saved[2].defined() ? OptTensor(saved[2]) : OptTensor(), (how & 1) != 0, (how & 2) == 0, stream);
+    if (q) out[0] = x[0];
+    if (k) out[1] = x[q ? 1 : 0];
+    return out;
+  }
+};
+
+std::tuple<Tensor, OptTensor> apply_rotary(const Tensor& q, const OptTensor& k, const Tensor& cos, const Tensor& sin,
+                                           const OptTensor& positions, bool half, int64_t stream) {
+  REFUSE_UNLESS(q.dim() == 4 && (!k || k->dim() == 4), "expected (B, H, T, D), got ", q.sizes(), k ? text(", ", k->sizes()) : "");
+  const int64_t B = q.size(0), T = q.size(2);
+  REFUSE_UNLESS(!k || (k->size(0) == B && k->size(2) == T && k->size(3) == q.size(3) && k->scalar_type() == q.scalar_type() &&
+                       k->device() == q.device()),
+                "q and k differ: ", q.sizes(), " ", q.scalar_type(), ", ", k ? text(k->sizes(), " ", k->scalar_type()) : "");
+  check_head_dim(q.size(3));
+  if (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kFloat)
+    throw py::type_error(text("apply_rotary takes bfloat16 or float32 inputs; got ", q.scalar_type()));
+  REFUSE_UNLESS(q.numel() > 0 && (!k || k->numel() > 0), "q and k must not be empty");
+  check_rotary_tables(cos, sin, q);
+  OptTensor at = positions;
+  if (positions) {
+    const Tensor& pos = *positions;
+    const bool one = pos.dim() == 1 && pos.size(0) == T, each = pos.dim() == 2 && pos.size(0) == B && pos.size(1) == T;
+    REFUSE_UNLESS((one || each) && (pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong), "positions must be int32 or "
+                  "int64 (", T, ",) or (", B, ", ", T, "), got ", pos.sizes(), " ", pos.scalar_type());
+    REFUSE_UNLESS(pos.device() == q.device(), "positions must be on ", q.device());
+    if (T > 1 && pos.stride(-1) != 1) at = pos.contiguous();
+  }
+  require_gpu(q);
+  const bool grad = c10::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()));
+  const auto x = grad ? RopeNode::apply(q, k, cos, sin, at, half, false, stream)
+                      : rope(q, k.value_or(Tensor()), cos, sin, at.value_or(Tensor()), half, false, stream);
+  return {x[0], k ? OptTensor(x[1]) : OptTensor()};
+}
+
+// A pool of one layer (dims 4) or of all layers (dims 5).
+void check_pool(const Tensor& k, const Tensor& v, int64_t dims) {
+  REFUSE_UNLESS(k.dim() == dims && v.dim() == dims, "k_pages and v_pages must have ", dims, " dimensions, got ", k.sizes(), ", ",
+                v.sizes());
+  bool match = k.size(dims - 1) == v.size(dims - 2) && k.size(dims - 2) == v.size(dims - 1);
+  for (int i = 0; i < dims - 2; ++i) match = match && k.size(i) == v.size(i);
+  REFUSE_UNLESS(match, "k_pages (.., pages, kv heads, page size, D) and v_pages (.., pages, kv heads, D, page size) do not match: ",
+                k.sizes(), ", ", v.sizes());
+  if (k.scalar_type() != v.scalar_type() || (k.scalar_type() != at::kBFloat16 && k.scalar_type() != at::kFloat8_e4m3fn))
+    throw py::type_error(text("the cache holds bfloat16 or float8_e4m3fn, got ", k.scalar_type(), " and ", v.scalar_type()));
+  REFUSE_UNLESS(k.is_contiguous() && v.is_contiguous(), "k_pages and v_pages must be contiguous");
+  REFUSE_UNLESS(k.device() == v.device(), "k_pages and v_pages must be on one device");
+  REFUSE_UNLESS(k.numel() > 0, "the pool must not be empty");
+}
+void check_scales(const Tensor& k_pages, const OptTensor& k_scale, const OptTensor& v_scale) {
+  if (k_pages.scalar_type() == at::kBFloat16) {
+    REFUSE_UNLESS(!k_scale && !v_scale, "a bfloat16 cache takes no scales");
+    return;
+  }
+  for (const OptTensor* t : {&k_scale, &v_scale})
+    REFUSE_UNLESS(*t && (*t)->scalar_type() == at::kFloat && (*t)->dim() == 1 && (*t)->size(0) == k_pages.size(1) &&
+                      (*t)->is_contiguous() && (*t)->device() == k_pages.device(),
+                  "an e4m3 cache needs ", t == &k_scale ? "k_scale" : "v_scale", ", contiguous float32 (", k_pages.size(1), ",) on ",
+                  k_pages.device());
+}
+void check_tokens(const char* what, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,
+                  const Tensor& lens, const OptTensor& counts, const OptTensor& k_scale, const OptTensor& v_scale) {
+  check_pool(k_pages, v_pages, 4);
+  REFUSE_UNLESS(q.dim() == 4, "expected (B, H, T, D), got ", q.sizes());
+  if (q.scalar_type() != at::kBFloat16) throw py::type_error(text(what, " takes bfloat16 heads; got ", q.scalar_type()));
+  check_head_dim(q.size(3));
+  REFUSE_UNLESS(q.numel() > 0, "q must not be empty");
+  REFUSE_UNLESS(q.size(3) == k_pages.size(3) && q.size(1) % k_pages.size(1) == 0, "q ", q.sizes(), " does not match the pool's ",
+                k_pages.size(1), " kv heads of ", k_pages.size(3), " values");
+  REFUSE_UNLESS(q.device() == k_pages.device(), "q is on ", q.device(), ", the pages on ", k_pages.device());
+  REFUSE_UNLESS(tables.dim() == 2 && tables.size(0) == q.size(0) && tables.size(1) > 0, "tables must be (", q.size(0),
+                ", entries), got ", tables.sizes());
+  check_ints("tables", tables, tables.sizes(), q);
+  check_ints("lens", lens, {q.size(0)}, q);
+  if (counts) check_ints("counts", *counts, {q.size(0)}, q);
+  check_scales(k_pages, k_scale, v_scale);
+  if (c10::GradMode::is_enabled() && q.requires_grad())
+    throw std::runtime_error(text(what, " is forward-only: call it under torch.no_grad() or on detached tensors"));
 }
 
 std::tuple<Tensor, OptTensor> paged_append(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& k_pages,
                                            const Tensor& v_pages, const Tensor& tables, const Tensor& lens,
-                                           const OptTensor& counts, const std::optional<double>& eps, const OptTensor& cos,
-                                           const OptTensor& sin, bool half, const OptTensor& k_scale,
+                                           const OptTensor& counts, const OptTensor& cos, const OptTensor& sin, bool half,
+                                           const std::optional<double>& eps, const OptTensor& k_scale,
                                            const OptTensor& v_scale, bool return_k, int64_t stream) {
+  check_tokens("paged_append", q0, k_pages, v_pages, tables, lens, counts, k_scale, v_scale);
+  for (const Tensor* t : {&k0, &v0}) {
+    REFUSE_UNLESS(t->dim() == 4 && t->size(0) == q0.size(0) && t->size(1) == k_pages.size(1) && t->size(2) == q0.size(2) &&
+                      t->size(3) == q0.size(3) && t->scalar_type() == q0.scalar_type() && t->device() == q0.device(),
+                  "k and v must be (", q0.size(0), ", ", k_pages.size(1), ", ", q0.size(2), ", ", q0.size(3), ") as q, got ",
+                  t->sizes(), " ", t->scalar_type());
+    if (c10::GradMode::is_enabled() && t->requires_grad())
+      throw std::runtime_error("paged_append is forward-only: call it under torch.no_grad() or on detached tensors");
+  }
+  REFUSE_UNLESS(cos.has_value() == sin.has_value(), "give both cos and sin, or neither");
+  if (cos) check_rotary_tables(*cos, *sin, q0);
+  REFUSE_UNLESS(!eps || *eps >= 0.0, "norm_eps must be non-negative");
+  require_gpu(q0);
   c10::DeviceGuard guard(q0.device());
   int64_t st[9];
   Tensor q = heads(q0, st), k = heads(k0, st + 3), v = heads(v0, st + 6);
@@ -449,8 +609,10 @@ std::tuple<Tensor, OptTensor> paged_append(const Tensor& q0, const Tensor& k0, c
 // out (B, H, T, D), a view of token-major storage, and the log-sum-exp when asked for.
 std::tuple<Tensor, OptTensor> paged_attention(const Tensor& q0, const Tensor& k_pages, const Tensor& v_pages,
                                               const Tensor& tables, const Tensor& lens, const OptTensor& counts,
-                                              int64_t window, double scale, const OptTensor& k_scale,
+                                              int64_t window, const std::optional<double>& scale, const OptTensor& k_scale,
                                               const OptTensor& v_scale, bool with_lse, int64_t stream) {
+  check_tokens("paged_attention", q0, k_pages, v_pages, tables, lens, counts, k_scale, v_scale);
+  require_gpu(q0);
   c10::DeviceGuard guard(q0.device());
   int64_t st[6];
   Tensor q = heads(q0, st);
@@ -463,46 +625,102 @@ std::tuple<Tensor, OptTensor> paged_attention(const Tensor& q0, const Tensor& k_
   if (need > 0) ws = workspace(q, need);
   check(flw_paged_attention(q.data_ptr(), st, k_pages.data_ptr(), v_pages.data_ptr(), cache_code(k_pages), k_pages.size(0), page,
                             i32(tables), tables.size(1), i32(lens), i32(counts), f32(k_scale), f32(v_scale), B, H, KV, T, D,
-                            window, (float)scale, out.data_ptr(), st + 3, f32(lse), opt(ws), need, str(stream)),
+                            window, (float)(scale ? *scale : 1.0 / std::sqrt((double)D)), out.data_ptr(), st + 3, f32(lse),
+                            opt(ws), need, str(stream)),
         "paged_attention");
   return {out.transpose(1, 2), lse};
 }
 
-Tensor reserve_pages(const Tensor& tables, const Tensor& lens, const Tensor& refs, const Tensor& counts, int64_t page,
-                     int64_t window, const Tensor& tables_out, const Tensor& lens_out, const Tensor& refs_out,
-                     int64_t stream) {
-  c10::DeviceGuard guard(tables.device());
+void check_state(const Tensor& tables, const Tensor& refs) {
+  REFUSE_UNLESS(tables.dim() == 2 && refs.dim() == 1 && tables.numel() > 0 && refs.numel() > 0,
+                "tables must be (S, entries) and refs (pages,), not empty, got ", tables.sizes(), ", ", refs.sizes());
+  check_ints("tables", tables, tables.sizes(), tables);
+  check_ints("refs", refs, refs.sizes(), tables);
+}
+// k_pages, v_pages of all layers (L, P, ..), or of one.
+std::pair<Tensor, Tensor> all_layers(const Tensor& k, const Tensor& v, const Tensor& refs) {
+  const bool one = k.dim() == 4 && v.dim() == 4;
+  std::pair<Tensor, Tensor> kv = one ? std::make_pair(k.unsqueeze(0), v.unsqueeze(0)) : std::make_pair(k, v);
+  check_pool(kv.first, kv.second, 5);
+  REFUSE_UNLESS(kv.first.size(1) == refs.size(0) && k.device() == refs.device(), "the pool ", k.sizes(), " on ", k.device(),
+                " is not of refs' ", refs.size(0), " pages");
+  return kv;
+}
+// The tensors to write: `out`, one for each input (each may be that input, but overlap no other), or new ones.
+std::vector<Tensor> outputs(const std::optional<std::vector<Tensor>>& out, const std::vector<Tensor>& in, const Tensor& arg) {
+  std::vector<Tensor> to;
+  if (!out) {
+    for (const Tensor& t : in) to.push_back(empty(t, t.sizes(), at::kInt));
+    return to;
+  }
+  REFUSE_UNLESS(out->size() == in.size(), "out takes ", in.size(), " tensors, got ", out->size());
+  auto overlap = [](const Tensor& a, const Tensor& b) {
+    return i32(a) < i32(b) + b.numel() && i32(b) < i32(a) + a.numel();
+  };
+  for (size_t i = 0; i < in.size(); ++i) {
+    const Tensor& o = (*out)[i];
+    check_ints("out", o, in[i].sizes(), in[i]);
+    bool bad = arg.defined() && overlap(o, arg);
+    for (size_t j = 0; j < in.size(); ++j)
+      bad = bad || (overlap(o, in[j]) && !(i == j && i32(o) == i32(in[j]))) || (j < i && overlap(o, (*out)[j]));
+    REFUSE_UNLESS(!bad, "an output may be its own input, and overlap nothing else");
+  }
+  return *out;
+}
+
+using OutTensors = std::optional<std::vector<Tensor>>;
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> reserve_pages(const Tensor& tables, const Tensor& lens, const Tensor& refs,
+                                                         const Tensor& counts, int64_t page, const std::optional<int64_t>& window,
+                                                         const OutTensors& out, int64_t stream) {
+  check_state(tables, refs);
   const int64_t S = tables.size(0), P = refs.size(0);
+  check_ints("lens", lens, {S}, tables);
+  check_ints("counts", counts, {S}, tables);
+  REFUSE_UNLESS(!window || *window > 0, "window must be positive");
+  require_gpu(tables);
+  const std::vector<Tensor> to = outputs(out, {tables, lens, refs}, counts);
+  c10::DeviceGuard guard(tables.device());
   Tensor granted = empty(lens, {S}, at::kInt), ws = workspace(lens, flw_reserve_pages_workspace_bytes(S, P));
-  check(flw_reserve_pages(i32(tables), i32(lens), i32(refs), i32(counts), S, tables.size(1), P, page, window, i32(tables_out),
-                          i32(lens_out), i32(refs_out), i32(granted), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
+  check(flw_reserve_pages(i32(tables), i32(lens), i32(refs), i32(counts), S, tables.size(1), P, page, window.value_or(0), i32(to[0]),
+                          i32(to[1]), i32(to[2]), i32(granted), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
         "reserve_pages");
-  return granted;
+  return {to[0], to[1], to[2], granted};
 }
 
-// k_pages, v_pages (L, P, KV, ..) as the two below take them.
-void reorder_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& lens, const Tensor& refs,
-                   const Tensor& parents, const Tensor& tables_out, const Tensor& lens_out, const Tensor& refs_out,
-                   int64_t stream) {
-  c10::DeviceGuard guard(tables.device());
+std::tuple<Tensor, Tensor, Tensor> reorder_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,
+                                                 const Tensor& lens, const Tensor& refs, const Tensor& parents,
+                                                 const OutTensors& out, int64_t stream) {
+  check_state(tables, refs);
   const int64_t S = tables.size(0), M = tables.size(1), P = refs.size(0);
+  check_ints("lens", lens, {S}, tables);
+  check_ints("parents", parents, {S}, tables);
+  const auto [k, v] = all_layers(k_pages, v_pages, refs);
+  require_gpu(tables);
+  const std::vector<Tensor> to = outputs(out, {tables, lens, refs}, parents);
+  c10::DeviceGuard guard(tables.device());
   Tensor ws = workspace(lens, flw_reorder_pages_workspace_bytes(S, M, P));
-  check(flw_reorder_pages(k_pages.data_ptr(), v_pages.data_ptr(), cache_code(k_pages), k_pages.size(0), P, k_pages.size(2),
-                          k_pages.size(3), k_pages.size(4), i32(tables), i32(lens), i32(refs), i32(parents), S, M,
-                          i32(tables_out), i32(lens_out), i32(refs_out), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
+  check(flw_reorder_pages(k.data_ptr(), v.data_ptr(), cache_code(k), k.size(0), P, k.size(2), k.size(3), k.size(4), i32(tables),
+                          i32(lens), i32(refs), i32(parents), S, M, i32(to[0]), i32(to[1]), i32(to[2]), ws.data_ptr(),
+                          (size_t)ws.numel(), str(stream)),
         "reorder_pages");
+  return {to[0], to[1], to[2]};
 }
 
-Tensor compact_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& refs,
-                     const Tensor& tables_out, const Tensor& refs_out, int64_t stream) {
-  c10::DeviceGuard guard(tables.device());
+std::tuple<Tensor, Tensor, Tensor> compact_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,
+                                                 const Tensor& refs, const OutTensors& out, int64_t stream) {
+  check_state(tables, refs);
+  const auto [k, v] = all_layers(k_pages, v_pages, refs);
+  require_gpu(tables);
   const int64_t P = refs.size(0);
+  const std::vector<Tensor> to = outputs(out, {tables, refs}, Tensor());
+  c10::DeviceGuard guard(tables.device());
   Tensor live = empty(refs, {1}, at::kInt), ws = workspace(refs, flw_compact_pages_workspace_bytes(P));
-  check(flw_compact_pages(k_pages.data_ptr(), v_pages.data_ptr(), cache_code(k_pages), k_pages.size(0), P, k_pages.size(2),
-                          k_pages.size(3), k_pages.size(4), i32(tables), i32(refs), tables.size(0), tables.size(1),
-                          i32(tables_out), i32(refs_out), i32(live), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
+  check(flw_compact_pages(k.data_ptr(), v.data_ptr(), cache_code(k), k.size(0), P, k.size(2), k.size(3), k.size(4), i32(tables),
+                          i32(refs), tables.size(0), tables.size(1), i32(to[0]), i32(to[1]), i32(live), ws.data_ptr(),
+                          (size_t)ws.numel(), str(stream)),
         "compact_pages");
-  return live;
+  return {to[0], to[1], live};
 }
 
 }  // namespace
@@ -540,7 +758,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("swiglu_bwd", &swiglu_bwd, nogil());
   m.def("act_quant_rows", &act_quant_rows, nogil());
   m.def("qkv_norm_rope_amax", &qkv_norm_rope_amax, nogil());
-  m.def("rope", &rope, nogil());
+  m.def("apply_rotary", &apply_rotary, nogil());
   m.def("paged_append", &paged_append, nogil());
   m.def("paged_attention", &paged_attention, nogil());
   m.def("reserve_pages", &reserve_pages, nogil());
