@@ -132,8 +132,8 @@ SIGNATURES = {
                                  c_int64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                  c_void_p, c_int, c_float, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p,
                                  c_void_p, c_void_p, c_void_p, c_void_p]),
-    "flw_paged_attention_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
-                                                       c_int64]),
+    "flw_paged_attention_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int64,
+                                                       c_int64, c_int64]),
     "flw_paged_attention": (c_int, [c_void_p, _P64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64,
                                     c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                                     c_int64, c_int64, c_float, c_void_p, _P64, c_void_p, c_void_p, c_size_t,

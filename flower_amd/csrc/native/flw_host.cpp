@@ -621,7 +621,7 @@ std::tuple<Tensor, OptTensor> paged_attention(const Tensor& q0, const Tensor& k_
   st[3] = T * H * D; st[4] = D; st[5] = H * D;
   OptTensor lse, ws;
   if (with_lse) lse = empty(q, {B, H, T}, at::kFloat);
-  const size_t need = flw_paged_attention_workspace_bytes(B, H, KV, T, D, page, tables.size(1), window);
+  const size_t need = flw_paged_attention_workspace_bytes(B, H, KV, T, D, cache_code(k_pages), page, tables.size(1), window);
   if (need > 0) ws = workspace(q, need);
   check(flw_paged_attention(q.data_ptr(), st, k_pages.data_ptr(), v_pages.data_ptr(), cache_code(k_pages), k_pages.size(0), page,
                             i32(tables), tables.size(1), i32(lens), i32(counts), f32(k_scale), f32(v_scale), B, H, KV, T, D,

@@ -496,8 +496,8 @@ int flw_paged_append(const void* q, const int64_t* q_strides, const void* k, con
  * rows 8-byte aligned; lse (B, H, T) fp32 (natural log of the sum of exp(scores); may be NULL). A padding token, and a query
  * without keys, gives zeros and an lse of -inf. fp32 softmax and sums. workspace: flw_paged_attention_workspace_bytes
  * (parts of long sequences; 0 where none is cut). */
-size_t flw_paged_attention_workspace_bytes(int64_t B, int64_t H, int64_t KV, int64_t T, int64_t D, int64_t page_size,
-                                           int64_t table_cols, int64_t window);
+size_t flw_paged_attention_workspace_bytes(int64_t B, int64_t H, int64_t KV, int64_t T, int64_t D, int cache_dtype,
+                                           int64_t page_size, int64_t table_cols, int64_t window);
 int flw_paged_attention(const void* q, const int64_t* q_strides, const void* k_pages, const void* v_pages, int cache_dtype,
                         int64_t num_pages, int64_t page_size, const int32_t* tables, int64_t table_cols, const int32_t* lens,
                         const int32_t* counts, const float* k_scale, const float* v_scale, int64_t B, int64_t H, int64_t KV,
