@@ -7,18 +7,23 @@
                            reference's torch op sequence; backward is the identity.
 ``causal_mask``         -- base.py:418-423, the boolean (T, T) band mask (plain torch).
 ``HeadRMSNorm``         -- base.py:341-357, parameter-free QK-norm (torch ops, the reference maths).
-``RotaryEmbedding``     -- base.py:436-483, RoPE with cached fp32 cos / sin tables.
+``RotaryEmbedding``     -- base.py:436-483, RoPE with cached fp32 cos / sin tables; and, beyond the
+                           reference, pairs half a rotation apart, a part of the head, and tables
+                           scaled for long contexts (``rotary_tables``), on the HIP rotary pass.
 ``CausalSelfAttention`` -- base.py:553-665 with the ``attn_precision`` switch (config.py:373):
                            "fp8" routes the heads through the FP8 sliding-window kernel, with the
                            QK-norm, RoPE and the e4m3 quantisation of Q/K/V fused in one HIP pass
                            pair (the reference's quantisation point, "after QK-norm and RoPE",
                            base.py:634-637) -- and, in training, through the differentiable FP8
                            attention (bf16 backward, straight-through quantisers); "bf16"
-                           through the HIP bf16 sliding-window kernel.
+                           through the HIP bf16 sliding-window kernel. ``forward_cached`` decodes
+                           over a ``PagedKVCache``.
 ``fp8_attention``       -- the FP8 route on (B, H, T, D) Q/K/V that are already normed and rotated.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.nn as nn
@@ -26,6 +31,7 @@ import torch.nn as nn
 from . import _lib
 from .kernels.fp8_swa_attention import (fp8_swa_attention, fp8_swa_attention_forward,
                                         fp8_swa_attention_from_codes, qk_norm_rope_quant_e4m3)
+from .kernels.rotary import ROTARY_LAYOUTS, apply_rotary
 from .kernels.swa_attention import swa_attention
 
 
@@ -183,22 +189,83 @@ class HeadRMSNorm(nn.Module):
         return (x.float() * rms).to(dtype=x.dtype)
 
 
+def rotary_tables(rotary_dim: int, positions: int, base: float = 10000.0, scaling: dict | None = None, device=None):
+    """(cos, sin) fp32 [positions, rotary_dim / 2] of position * f_i, f_i = base^(-2 i / rotary_dim); the angles in 64 bits.
+
+    scaling, for contexts longer by ``factor`` than those trained on:
+      {"type": "linear", "factor": s}     f_i / s (positions interpolated);
+      {"type": "ntk", "factor": s}        the base grown to base * s^(R / (R - 2)), so that the slowest pair is slower by s
+                                          and the fastest as it was;
+      {"type": "yarn", "factor": s, "original_positions": L, "beta_fast": 32, "beta_slow": 1, "attention_factor": None}
+                                          pairs that turn more than beta_fast times in L positions keep f_i, those that turn
+                                          less than beta_slow times get f_i / s, a line over i in between; both tables times
+                                          the attention factor, 0.1 ln s + 1 by default.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2 != 0:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    scaling = dict(scaling or {"type": "none"})
+    kind, factor, gain = scaling.pop("type", None), float(scaling.pop("factor", 1.0)), 1.0
+    if kind not in ("none", "linear", "ntk", "yarn") or not factor >= 1.0:
+        raise ValueError(f"scaling must be linear|ntk|yarn with a factor of 1 or more, got {kind!r}, {factor}")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    if kind == "ntk" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = float(base) ** (-i / rotary_dim)
+    if kind == "linear":
+        freq = freq / factor
+    elif kind == "yarn":
+        length = scaling.pop("original_positions", None)
+        fast, slow = float(scaling.pop("beta_fast", 32.0)), float(scaling.pop("beta_slow", 1.0))
+        gain = scaling.pop("attention_factor", None)
+        if length is None or length <= 0 or not fast > slow > 0.0:
+            raise ValueError("yarn takes original_positions, and beta_fast > beta_slow > 0")
+        gain = 0.1 * math.log(factor) + 1.0 if gain is None else float(gain)
+
+        def pair(turns: float) -> float:                 # the (fractional) pair that turns so often in `length` positions
+            return rotary_dim * math.log(length / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
+
+        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rotary_dim // 2 - 1)
+        slower = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        freq = freq * (1.0 - slower) + freq / factor * slower
+    if scaling:
+        raise ValueError(f"unknown {kind} scaling options {sorted(scaling)}")
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * freq
+    return tuple((t * gain).to(device=device, dtype=torch.float32) for t in (angle.cos(), angle.sin()))
+
+
 class RotaryEmbedding(nn.Module):
     """RoPE with cached cos / sin tables (base.py:436-483): pairs (2i, 2i+1) rotate by
     position * base^(-2i / head_dim); the fp32 tables are built once on the CPU and cast to the
     activations' dtype at use, as the reference does, so the fused kernel and the torch path see
-    the same table values."""
+    the same table values.
 
-    def __init__(self, head_dim: int, max_seq_len: int, base: float = 10000.0) -> None:
+    layout "half" (pairs (i, i + rotary_dim / 2)), rotary_dim (the head's first values turn, the rest
+    stays) and scaling (as ``rotary_tables`` takes it) go beyond the reference: with any of them
+    (``plain`` False) the tables are ``rotary_tables``' in fp32 and the rotation is ``apply_rotary``,
+    on the GPU."""
+
+    def __init__(self, head_dim: int, max_seq_len: int, base: float = 10000.0, *, layout: str = "interleaved",
+                 rotary_dim: int | None = None, scaling: dict | None = None) -> None:
         super().__init__()
         if head_dim % 2 != 0:
             raise ValueError("RoPE requires even head_dim")
+        if layout not in ROTARY_LAYOUTS:
+            raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        self.plain = layout == "interleaved" and rotary_dim == head_dim and scaling is None
+        if not self.plain and not (0 < rotary_dim <= head_dim and rotary_dim % 8 == 0):
+            raise ValueError(f"rotary_dim must be a multiple of 8 up to the head_dim {head_dim}, got {rotary_dim}")
+        self.layout, self.rotary_dim, self._scaling = layout, rotary_dim, scaling
         self._base = base
         self._head_dim = head_dim
-        cos, sin = self._tables(max_seq_len)
+        self._max_seq_len = max_seq_len
+        cos, sin = self._tables(max_seq_len) if self.plain else (None, None)
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
         self._cast = {}
+        self._pairs = {}
+        if not self.plain:
+            rotary_tables(rotary_dim, 1, base, scaling)  # refuses what it cannot scale
 
     def _tables(self, seq_len: int):
         inv_freq = 1.0 / (self._base ** (torch.arange(0, self._head_dim, 2).float() / self._head_dim))
@@ -222,6 +289,8 @@ class RotaryEmbedding(nn.Module):
 
     def tables(self, seq_len: int, dtype: torch.dtype, device) -> tuple[torch.Tensor, torch.Tensor]:
         """(cos, sin) as contiguous [seq_len, head_dim] tensors of ``dtype`` on ``device``."""
+        if not self.plain:
+            raise ValueError("tables of whole interleaved heads are for plain RoPE: use pair_tables")
         if seq_len > self.cos.shape[-2]:
             self._extend_cache(seq_len)
         key = (seq_len, dtype, torch.device(device), self.cos.data_ptr())
@@ -231,7 +300,28 @@ class RotaryEmbedding(nn.Module):
             self._cast = {key: hit}
         return hit
 
+    def pair_tables(self, seq_len: int, dtype: torch.dtype, device) -> tuple[torch.Tensor, torch.Tensor]:
+        """(cos, sin) fp32 [seq_len, rotary_dim / 2] for ``apply_rotary`` and ``paged_append``: the values that ``forward``
+        multiplies heads of ``dtype`` by (plain: rounded to it)."""
+        if not self.plain:                               # fp32 whatever the module is cast to
+            hit = self._pairs.get(torch.device(device))
+            if hit is None or hit[0].shape[0] < seq_len:
+                hit = rotary_tables(self.rotary_dim, max(seq_len, self._max_seq_len), self._base, self._scaling, device)
+                self._pairs = {torch.device(device): hit}
+            return hit[0][:seq_len], hit[1][:seq_len]
+        if seq_len > self.cos.shape[-2]:
+            self._extend_cache(seq_len)
+        key = (seq_len, dtype, torch.device(device), self.cos.data_ptr())
+        hit = self._pairs.get(key)
+        if hit is None:
+            hit = tuple(t[0, 0, :seq_len, ::2].to(device=device, dtype=dtype).float().contiguous() for t in (self.cos, self.sin))
+            self._pairs = {key: hit}
+        return hit
+
     def forward(self, q: torch.Tensor, k: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        if not self.plain:
+            cos, sin = self.pair_tables(q.shape[-2], q.dtype, q.device)
+            return apply_rotary(q, k, cos, sin, layout=self.layout)
         cos, sin = self.tables(q.shape[-2], q.dtype, q.device)
         return q * cos + self._rotate_half(q) * sin, k * cos + self._rotate_half(k) * sin
 
@@ -259,6 +349,9 @@ class CausalSelfAttention(nn.Module):
     ``fused_fp8_qkv`` (False): with a tensorwise Fp8Linear ``qkv`` in training, run the projection
     and the heads pass as one node whose backward hands |dqkv|'s maximum to the gradient cast
     (``_Fp8QkvHeadsFn``; the same results bit for bit).
+    ``rope_layout`` ("interleaved"), ``rope_dim`` (the head) and ``rope_scaling`` (None): RotaryEmbedding's
+    options beyond the reference; with any of them the heads are split and normed in torch and turned by
+    ``apply_rotary``, in every route.
     """
 
     fused_fp8_qkv = False
@@ -278,7 +371,9 @@ class CausalSelfAttention(nn.Module):
         self.attn_precision = precision
         self.fp8_granularity = getattr(config, "fp8_attention_granularity", "head")
         self.rope = RotaryEmbedding(self.head_dim, getattr(config, "max_seq_len", 8192),
-                                    base=getattr(config, "rope_base", 10000.0))
+                                    base=getattr(config, "rope_base", 10000.0),
+                                    layout=getattr(config, "rope_layout", "interleaved"),
+                                    rotary_dim=getattr(config, "rope_dim", None), scaling=getattr(config, "rope_scaling", None))
         bias = bool(getattr(config, "use_bias", True))
         self.qkv = nn.Linear(config.d_model, config.d_model * 3, bias=bias)
         self.out = nn.Linear(config.d_model, config.d_model, bias=bias)
@@ -306,7 +401,7 @@ class CausalSelfAttention(nn.Module):
                 q, k, v = _fake_quant_e4m3(q), _fake_quant_e4m3(k), _fake_quant_e4m3(v)
             return q, k, v
         y = self.qkv(x)
-        if y.is_cuda and y.dtype == torch.bfloat16 and self.head_dim in (32, 64, 128):
+        if self.rope.plain and y.is_cuda and y.dtype == torch.bfloat16 and self.head_dim in (32, 64, 128):
             cos, sin = self.rope.tables(y.shape[1], y.dtype, y.device)
             eps = self.qk_norm.eps if self.qk_norm is not None else 0.0
             q, k, v = _QkvHeadsFn.apply(y, self.num_heads, self.qk_norm is not None, eps, cos, sin)
@@ -330,7 +425,7 @@ class CausalSelfAttention(nn.Module):
         what the amax pass it spares the gradient cast costs, with a fold launch besides."""
         from .precision import Fp8Linear
         m = self.qkv
-        return (self.fused_fp8_qkv and type(m) is Fp8Linear and m.recipe == "tensorwise" and getattr(m, "backward_fp8", True)
+        return (self.fused_fp8_qkv and self.rope.plain and type(m) is Fp8Linear and m.recipe == "tensorwise" and getattr(m, "backward_fp8", True)
                 and m.bias is None and m.in_features % 16 == 0 and m.out_features % 16 == 0
                 and x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 3 and x.numel() > 0
                 and not torch.is_autocast_enabled() and self.head_dim in (32, 64, 128)
@@ -350,7 +445,7 @@ class CausalSelfAttention(nn.Module):
         if self.attn_precision == "fp8":
             if self._needs_grad(x):
                 return self._forward_fp8_train(x)
-            return self._forward_fp8(x, trace)
+            return self._forward_fp8(x, trace) if self.rope.plain else self.forward_unfused(x)
         q, k, v = self.qkv_heads(x)
         # token-major O: the transpose back to [B, T, H D] rows below is a view, in both directions
         out = swa_attention(q, k, v, self._window(x.shape[1]), token_major=q.dtype == torch.bfloat16)
@@ -384,4 +479,34 @@ class CausalSelfAttention(nn.Module):
             return self._forward_fp8_train(x)
         q, k, v = self.qkv_heads(x)
         out = fp8_swa_attention_forward(q, k, v, self._window(x.shape[1]), granularity=self.fp8_granularity)
+        return self.out(out.transpose(1, 2).reshape(x.shape))
+
+    @torch.no_grad()
+    def forward_cached(self, x: torch.Tensor, cache, layer: int, *, prompt: bool = False) -> torch.Tensor:
+        """The new tokens x (B, T, d), bf16, of the B sequences of ``cache`` (a PagedKVCache, in which ``reserve`` has made
+        room for them: counts[b] of sequence b's T tokens are new, the rest is padding) through this layer: qkv, then one HIP
+        pass that norms and turns q and k and writes k and v to the cache's pages, then attention over the pages, then
+        ``out``. T = 1 decodes; a longer T continues a prompt, or checks drafted tokens. Forward-only; ``attn_precision``
+        does not enter: the cache's type does.
+
+        prompt: the tokens are all that their sequences hold (a first prompt): they attend to each other by the bf16
+        sliding-window kernel, as fast as ``forward``, instead of over the pages (and to their keys and values as they were
+        before an e4m3 cache's cast). Padding tokens' rows then hold no meaning (else: what ``out`` makes of zeros), and
+        their x must be finite.
+        """
+        if x.dim() != 3 or x.shape[0] != cache.sequences:
+            raise ValueError(f"x must be ({cache.sequences}, T, d), got {tuple(x.shape)}")
+        if self.fp8_attention_sim:
+            raise ValueError("fp8_attention_sim takes its scales from whole sequences: it has no cached form")
+        if cache.window is not None and (self.local_window is None or self.local_window > cache.window):
+            raise ValueError(f"the cache keeps a window of {cache.window} positions, this layer sees {self.local_window}")
+        q, k, v = (self._split(t) for t in self.qkv(x).chunk(3, dim=-1))
+        cos, sin = self.rope.pair_tables(cache.max_len, q.dtype, q.device)
+        how = dict(cos=cos, sin=sin, layout=self.rope.layout, norm_eps=self.qk_norm.eps if self.qk_norm is not None else None)
+        if prompt:
+            q, k = cache.append(layer, q, k, v, return_k=True, **how)
+            out = swa_attention(q, k, v.contiguous(), self._window(x.shape[1]), token_major=True)
+        else:
+            q = cache.append(layer, q, k, v, **how)
+            out = cache.attend(layer, q, window=self.local_window)
         return self.out(out.transpose(1, 2).reshape(x.shape))

@@ -491,6 +491,18 @@ class TransformerBlock(nn.Module):
         x = x + self.ff(self.ln2(x))
         return x, memory
 
+    @torch.no_grad()
+    def forward_cached(self, x: torch.Tensor, cache, layer: int, *, prompt: bool = False) -> torch.Tensor:
+        """The new tokens x (B, T, d) through the block, their keys and values into layer ``layer`` of ``cache``
+        (``CausalSelfAttention.forward_cached``). Forward-only."""
+        a = self.attn.forward_cached(self.ln1(x), cache, layer, prompt=prompt)
+        d = x.shape[-1]
+        if d % 8 == 0 and d <= 8192 and x.numel() > 0 and _hip_rows_ok(x, a, self.ln2.weight):
+            x, h = _AddRMSNormFn.apply(x, a, self.ln2.weight, self.ln2.eps)
+            return self.ff(h, residual=x)
+        x = x + a
+        return x + self.ff(self.ln2(x))
+
 
 def block_config(**overrides) -> SimpleNamespace:
     """The 450M ``vanilla_matched`` block (configs/sweep13_450m_longctx_fp8.yaml:94-113): d_model

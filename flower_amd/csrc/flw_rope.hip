@@ -239,10 +239,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
         for (int j = 0; j < 8; ++j) f[j] *= r;
       }
       unit.turn(f);
-      if (w == 0) {
-        if (!live)
+      if (!live)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = 0.0f;
+        for (int j = 0; j < 8; ++j) f[j] = 0.0f;
+      if (w == 0) {
         unit_store(p.q_out + (((int64_t)b * p.H + h) * p.T + t) * D, at, f);
         continue;
       }

@@ -35,7 +35,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
 
     q (B, H, T, D), k and v (B, KV, T, D) bf16, any strides with contiguous 16-byte rows (views of a projection's output).
     Token t of sequence b stands at position lens[b] - counts[b] + t (``lens`` counts the new tokens in; ``counts`` None: T
-    each); tokens t >= counts[b] are padding: nothing is written for them and their q' is zero. norm_eps: q and k are normed
+    each); tokens t >= counts[b] are padding: nothing is written for them and their q' (and k') is zero. norm_eps: q and k are normed
     over the head first (x / sqrt(mean(x^2) + eps), HeadRMSNorm). cos, sin, layout: rotary positions as in ``apply_rotary``.
     fp32 arithmetic, rounded once. A position without a page is not written. Forward-only.
     """
@@ -56,8 +56,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     i = lens[b] - counts[b] + t and sees the keys j <= i, with i - j < window when a window is given (window <= 0: none, the
     result is zero). H is a multiple of the pool's kv heads: query head h reads kv head h // (H / KV). scale: of the scores,
     1 / sqrt(D) by default. A query without keys, and a padding token, gives zeros (lse -inf). Softmax and sums in fp32; an
-    e4m3 cache's codes are multiplied as they are. Made for few tokens a sequence (T H / KV up to 16 read the cache once;
-    each further 16 read it again). Forward-only.
+    e4m3 cache's codes are multiplied as they are. Made for few tokens a sequence: up to 64 rows (T H / KV) of a kv head read
+    the cache once, each further 64 read it again. Forward-only.
     """
     out, lse = _lib.native().paged_attention(q, k_pages, v_pages, tables, lens, counts, _FULL if window is None else window,
                                              scale, k_scale, v_scale, return_lse, _lib.stream_or_none(q))

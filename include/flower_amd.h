@@ -482,7 +482,7 @@ int flw_rope(const void* q, const int64_t* q_strides, int64_t H, const void* k, 
  * HeadRMSNorm, flower/models/base.py:341-357), turned by their positions when cos / sin are given (flw_rope's tables and
  * layouts), k and v written to their pages (e4m3: rne(clamp(x / scale, +-448)), NaN kept). fp32 arithmetic, rounded once.
  * q (B, H, T, D), k, v (B, KV, T, D) bf16, strides {b, h, t}, 16-byte aligned rows; q_out contiguous (B, H, T, D), zero for
- * padding; k_out (contiguous (B, KV, T, D) bf16, the k that was written) may be NULL. */
+ * padding; k_out (contiguous (B, KV, T, D) bf16, the k that was written, zero for padding) may be NULL. */
 int flw_paged_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                      const int64_t* v_strides, int64_t B, int64_t H, int64_t KV, int64_t T, int64_t D, void* k_pages,
                      void* v_pages, int cache_dtype, int64_t num_pages, int64_t page_size, const int32_t* tables,

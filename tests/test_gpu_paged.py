@@ -98,6 +98,12 @@ ATTENTION = [
     (1, 1, 1, 64, 1024, "bf16", [9000], None, None),
     (1, 4, 1, 64, 64, "bf16", [20000], None, None),                 # cut into parts
     (1, 4, 2, 128, 64, "e4m3", [20001, 3], None, None),
+    (1, 4, 6, 64, 64, "bf16", [3000, 9, 1500], [6, 6, 0], None),    # two, four waves of rows, whole items and parts
+    (1, 4, 5, 128, 16, "bf16", [2100, 700], None, 1900),
+    (2, 8, 5, 128, 16, "e4m3", [2100, 5], [5, 2], None),
+    (1, 8, 8, 64, 32, "e4m3", [1500], None, 1000),
+    (1, 6, 16, 32, 64, "bf16", [1200, 40], [16, 11], None),         # two groups of rows
+    (1, 8, 16, 128, 128, "bf16", [1100], None, 600),
 ]
 
 
