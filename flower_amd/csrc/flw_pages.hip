@@ -268,53 +268,50 @@ struct PageCopy {
   const int32_t* pairs;           // reorder: [S][3]; compact: [2][P] dst then src
   const int32_t* count;           // compact: pairs in use
   int64_t P;
-  int L, KV, D, page, size;       // size: bytes a value
+  int S, L, KV, D, page, size;    // S: reorder; size: bytes a value
 };
 
-// Reorder: the first `used` positions of page src to page dst; one workgroup a (place, layer, k or v, kCopyHeads heads). A
-// thread takes one 16-byte run of a head's page, of each of the heads: their loads are in flight together.
-constexpr int kCopyHeads = 4;
+// 16 bytes that are read (written) once: past the caches (reorder's copies 56 us with such stores alone, 51 with both).
+typedef uint32_t Run __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ Run run_load(const uint8_t* p) { return __builtin_nontemporal_load(reinterpret_cast<const Run*>(p)); }
+__device__ __forceinline__ void run_store(uint8_t* p, Run x) { __builtin_nontemporal_store(x, reinterpret_cast<Run*>(p)); }
+
+// Reorder: the first `used` positions of page src to page dst; one workgroup a (place, k or v, layer, head), a thread a 16-byte
+// run at a time. The places are the grid's slow side and k / v its next one: workgroups go to the eight XCDs by their number
+// modulo 8, so that with places, or k / v, on the fast side a regular pattern of forks, or v's partly written lines, fell to half
+// of them. 32 forks of 47 tokens in 12 layers of 20 heads of 64 (184 MB read and written): 45 us, 4.1 TB/s; places fast 70, k / v
+// fast 51. Two heads a thread the same, four 48; whole 64-byte pieces written (with what dst held) 57.
+constexpr int kCopyRows = 32768;
 __global__ __launch_bounds__(256) void copy_tail_kernel(PageCopy p) {
-  const int s = blockIdx.x;
+  const int s = blockIdx.y + kCopyRows * blockIdx.z;
+  if (s >= p.S) return;
   const int32_t dst = p.pairs[3 * s], src = p.pairs[3 * s + 1];
   if (dst < 0) return;
-  const int used = p.pairs[3 * s + 2];
-  const int groups = (p.KV + kCopyHeads - 1) / kCopyHeads;
-  const int of = (int)blockIdx.y >> 1, layer = of / groups, h0 = (of - layer * groups) * kCopyHeads;
-  const int nh = p.KV - h0 < kCopyHeads ? p.KV - h0 : kCopyHeads;
+  const int half = (int)gridDim.x >> 1;     // layers x heads
+  const bool rows = (int)blockIdx.x >= half;
+  const int64_t of = (int)blockIdx.x - (rows ? half : 0), layer = of / p.KV, head = of - layer * p.KV;
   const int64_t bytes = (int64_t)p.page * p.D * p.size;
-  uint8_t* pool = blockIdx.y & 1 ? p.v : p.k;
-  const uint8_t* a = pool + (((int64_t)layer * p.P + src) * p.KV + h0) * bytes;
-  uint8_t* b = pool + (((int64_t)layer * p.P + dst) * p.KV + h0) * bytes;
-  const bool rows = blockIdx.y & 1;
-  // k: `used` rows of D values, a whole number of runs. v: of each of D rows the first `used` values; `per` runs a row.
-  const int lper = __builtin_ctz((unsigned)(p.page * p.size / 16)), per = 1 << lper;
-  const int n = rows ? p.D << lper : used * p.D * p.size / 16, fill = used * p.size;
+  uint8_t* pool = rows ? p.v : p.k;
+  const uint8_t* a = pool + ((layer * p.P + src) * p.KV + head) * bytes;
+  uint8_t* b = pool + ((layer * p.P + dst) * p.KV + head) * bytes;
+  // k: `used` rows of D values, a whole number of runs. v: of each of D rows the first `used` values, in `per` runs.
+  const int fill = p.pairs[3 * s + 2] * p.size, per = (fill + 15) / 16, n = rows ? p.D * per : p.D * fill / 16;
+  const uint32_t by_per = (uint32_t)((0x100000000ull + (unsigned)per - 1) / (unsigned)per);      // i / per = i by_per >> 32
   for (int i = threadIdx.x; i < n; i += 256) {
-    const int left = rows ? fill - 16 * (i & (per - 1)) : 16;
-    if (left <= 0) continue;
-    uint4 x[kCopyHeads];
+    const int row = per == 1 ? i : (int)__umulhi((uint32_t)i, by_per), run = i - row * per;
+    const int left = rows ? fill - 16 * run : 16;
+    const int64_t at = rows ? (int64_t)row * p.page * p.size + 16 * run : 16 * (int64_t)i;
+    Run x = run_load(a + at);
+    if (left < 16) {                        // the row's last run: what lies behind `used` stays (its one writer is this thread)
+      const Run was = *reinterpret_cast<const Run*>(b + at);      // (its line stays in L2 for the stores: not so 75 us)
 #pragma unroll
-    for (int h = 0; h < kCopyHeads; ++h)
-      if (h < nh) x[h] = *reinterpret_cast<const uint4*>(a + h * bytes + 16 * (int64_t)i);
-#pragma unroll
-    for (int h = 0; h < kCopyHeads; ++h) {
-      if (h >= nh) continue;
-      uint4* to = reinterpret_cast<uint4*>(b + h * bytes + 16 * (int64_t)i);
-      if (left < 16) {                     // the row's last run: what lies behind `used` stays (its one writer is this thread)
-        const uint4 was = *to;
-        uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
-        const uint32_t o[4] = {was.x, was.y, was.z, was.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = left - 4 * e;                          // bytes of this word to take
-          const uint32_t m = k >= 4 ? 0xFFFFFFFFu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
-          w[e] = (w[e] & m) | (o[e] & ~m);
-        }
-        x[h] = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int e = 0; e < 4; ++e) {
+        const int k = left - 4 * e;         // bytes of this word to take
+        const uint32_t m = k >= 4 ? 0xFFFFFFFFu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
+        x[e] = (x[e] & m) | (was[e] & ~m);
       }
-      *to = x[h];
     }
+    run_store(b + at, x);
   }
 }
 
@@ -334,7 +331,7 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(PageCopy p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int e = (int)threadIdx.x + 256 * j;
-      if (e < m) reinterpret_cast<uint4*>(b)[e] = reinterpret_cast<const uint4*>(a)[e];
+      if (e < m) run_store(b + 16 * e, run_load(a + 16 * e));
     }
   }
 }
@@ -495,11 +492,13 @@ extern "C" int flw_reorder_pages(void* k_pages, void* v_pages, int cache_dtype, 
   PageCopy c{};
   c.k = static_cast<uint8_t*>(k_pages); c.v = static_cast<uint8_t*>(v_pages); c.pairs = p.pairs; c.P = num_pages;
   c.L = (int)L; c.KV = (int)KV; c.D = (int)D; c.page = (int)page_size; c.size = cache_dtype == FLW_E4M3 ? 1 : 2;
+  c.S = (int)S;
+  const dim3 grid((unsigned)(2 * L * KV), (unsigned)(S < kCopyRows ? S : kCopyRows),
+                  (unsigned)((S + kCopyRows - 1) / kCopyRows));
   const Timer tm = take_timer();
   (void)launch_ext(reinterpret_cast<const void*>(&reorder_rows_kernel), dim3((unsigned)S), dim3(256), 0, s, p, tm.start, nullptr);
   (void)launch_ext(reinterpret_cast<const void*>(&reorder_take_kernel), dim3(1), dim3(kScan), 0, s, p, nullptr, nullptr);
-  (void)launch_ext(reinterpret_cast<const void*>(&copy_tail_kernel), dim3((unsigned)S, (unsigned)(2 * L * ((KV + kCopyHeads - 1) / kCopyHeads))),
-                   dim3(256), 0, s, c, nullptr, tm.stop);
+  (void)launch_ext(reinterpret_cast<const void*>(&copy_tail_kernel), grid, dim3(256), 0, s, c, nullptr, tm.stop);
   return check_launch("flw_reorder_pages");
 }
 
