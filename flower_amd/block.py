@@ -298,6 +298,13 @@ class Fp8DecoderBlock(nn.Module):
         x = x + self.attn.forward_unfused(self.ln1(x))
         return x + self.ff(self.ln2(x))
 
+    @torch.no_grad()
+    def forward_cached(self, x: torch.Tensor, cache, layer: int, *, prompt: bool = False) -> torch.Tensor:
+        """The new tokens x (B, T, d) through the block, their keys and values into layer ``layer`` of ``cache``
+        (``CausalSelfAttention.forward_cached``; the attention in the cache's type, the linears in FP8)."""
+        x = x + self.attn.forward_cached(self.ln1(x), cache, layer, prompt=prompt)
+        return x + self.ff(self.ln2(x))
+
     def _linears(self):
         return self.attn.qkv, self.attn.out, self.ff.net[0], self.ff.net[3]
 

@@ -260,6 +260,22 @@ def test_the_block_decodes_as_it_prompts():
     assert float((got - want).abs().max()) <= (1 + 4) * 2.0 ** -6 * float(want.abs().max())
 
 
+def test_the_fp8_block_decodes():
+    """Fp8DecoderBlock over the cache: the composition of its modules, bit for bit, prompt and decode; one token a call or
+    several, a row's result is the same to the attention's own rounding (per-row activation scales)."""
+    from flower_amd.block import Fp8DecoderBlock
+    torch.manual_seed(1)
+    b = Fp8DecoderBlock(128, 2, 256, 24).cuda().bfloat16().eval()
+    x = seeded((4, 30, 128), 8, torch.bfloat16)
+    cache, twin = make_cache(1), make_cache(1)
+    with torch.no_grad():
+        for t0, t1 in ((0, 20), (20, 21), (21, 25)):
+            cache.reserve(t1 - t0), twin.reserve(t1 - t0)
+            got = b.forward_cached(x[:, t0:t1], cache, 0, prompt=t0 == 0)
+            h = x[:, t0:t1] + b.attn.forward_cached(b.ln1(x[:, t0:t1]), twin, 0, prompt=t0 == 0)
+            assert torch.equal(got, h + b.ff(b.ln2(h))) and bool(torch.isfinite(got).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
 def test_captured_decode_steps_replay_as_eager_ones(dtype):
     """Two graphs of whole decode steps (pages reserved, two blocks, with a beam reorder in the one), each with a cache of
