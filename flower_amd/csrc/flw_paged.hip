@@ -20,12 +20,13 @@
 // sum and O are fp32.
 // e4m3 pages: codes widened to bf16 in registers (exact); the K scale multiplies the score, the V scale the output.
 //
-// Work: an item is a (sequence, row group, kv head), its length the blocks of its key range. Either a workgroup an item, or the
-// blocks of all items laid end to end and cut into equal parts, one for each workgroup that the GPU holds; an item cut by a border
-// leaves fp32 partial results, which a second launch joins. A workgroup begins an item's loads while it ends the one before.
+// Work: an item is a (sequence, row group, kv head), its length the blocks of its key range. Either a workgroup an item (of one
+// row tile: a wave, or four that take a quarter of its blocks each and join in LDS), or the blocks of all items laid end to end
+// and cut into equal parts, one for each workgroup that the GPU holds; an item cut by a border leaves fp32 partial results, which
+// a second launch joins. A workgroup begins an item's loads while it ends the one before.
 //
 // Measured: 64 sequences of up to 2048 keys, 20 heads of 64: 103 us, 5.9 TB/s of K and V. 4 sequences of 70 001 to 131 072 keys, 32
-// heads on 4 of 128: 138 us, 5.9 TB/s. Short calls are latency: 100 keys of 16 heads take 6.4 us, most of it the first fetch of
+// heads on 4 of 128: 138 us, 5.9 TB/s. Short calls are latency: 100 keys of 16 heads take 5.9 us, most of it the first fetch of
 // the code and of the page numbers, the lengths and the keys that depend on each other.
 
 #include <utility>
@@ -359,12 +360,16 @@ struct PaPart {
   int lo, hi, kb, blocks;
 };
 
-template <int D, bool F8, bool WIDE, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? (D == 128 && !F8 ? 2 : 3) : 2) void paged_attn_kernel(PagedAttn p) {
+// SPLIT > 1: that many waves a workgroup, each on its own as with WAVES = 1, share the blocks of one item and join in LDS.
+template <int D, bool F8, bool WIDE, int WAVES, int SPLIT = 1>
+__global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES == 4 ? (D == 128 && !F8 ? 2 : 3) : 2) void paged_attn_kernel(PagedAttn p) {
   using Blk = PaBlock<D, F8, WIDE, WAVES>;
   constexpr int DT = Blk::DT, KS = Blk::KS, NI = Blk::NI, TILE = Blk::TILE, ROWS = 16 * WAVES;
   constexpr int BUFS = Blk::BUFS, AHEAD = WAVES > 1 ? 1 : BUFS;
-  __shared__ __align__(1024) uint8_t ring[Blk::RING];
+  static_assert(WAVES == 1 || SPLIT == 1);
+  __shared__ __align__(1024) uint8_t rings[SPLIT * Blk::RING];
+  const int sw = SPLIT == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  uint8_t* ring = rings + sw * Blk::RING;
   const PaWave<D, F8, WIDE, WAVES> wv(p, ring);
   const int n = wv.n, g = wv.g;
   const int me = (int)blockIdx.x, pairs = p.B * p.groups;
@@ -379,6 +384,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? (D == 128 && !F8 ? 2 : 3) 
     pair = pa_div(me, p.by_kv);
     kvh = me - pair * p.KV;
     to = total = per = range(pair).blocks();
+    if constexpr (SPLIT > 1) {
+      cur = to * sw / SPLIT;
+      to = to * (sw + 1) / SPLIT;
+    }
   } else {
     int upto = 0, mine = 0, from = 0;
     pair = 0;
@@ -427,7 +436,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? (D == 128 && !F8 ? 2 : 3) 
   auto part_of = [&](const PaRange& rg) __attribute__((always_inline)) {
     const int e = s + rg.blocks(), end = e < to ? e : to;
     return PaPart{p.tables + (int64_t)pa_div(pair, p.by_groups) * p.M, (int64_t)kvh * (Blk::RB << p.shift), rg.lo, rg.hi,
-                  rg.kb_lo + (cur - s), s >= to ? -1 : rg.kb_hi > rg.kb_lo ? end - cur : 0};
+                  rg.kb_lo + (cur - s), SPLIT == 1 && s >= to ? -1 : rg.kb_hi > rg.kb_lo ? end - cur : 0};
   };
   PaRange rg = range(pair);
   PaPart at = part_of(rg);
@@ -437,7 +446,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? (D == 128 && !F8 ? 2 : 3) 
   for (int nth = 0; at.blocks >= 0; ++nth) {
     const int b = pa_div(pair, p.by_groups), group = pair - b * p.groups, kv = kvh, item = pair * p.KV + kvh;
     const int from_s = s, e = s + rg.blocks();
-    const bool begins = cur == s, ends = at.blocks == 0 || cur + at.blocks == e;
+    const bool begins = cur == s, ends = SPLIT > 1 || at.blocks == 0 || cur + at.blocks == e;
     // the part after this one
     PaRange nrg = rg;
     PaPart nx = at;
@@ -678,7 +687,38 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? (D == 128 && !F8 ? 2 : 3) 
     float* part = p.part + (2ll * me + (nth > 0)) * (ROWS * (D + 2));      // (whole: not used)
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    if (r < rg.here) {
+    if constexpr (SPLIT > 1) {
+      constexpr int SLOT = 16 * (D + 2);
+      static_assert(4 * SLOT <= Blk::RING);
+      float* mine = reinterpret_cast<float*>(ring);       // (this wave is done with its blocks)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<float4*>(mine + r * D + 16 * dt + 4 * g) = make_float4(acc[dt][0], acc[dt][1], acc[dt][2], acc[dt][3]);
+      if (g == 0) {
+        mine[16 * D + r] = m;
+        mine[16 * D + 16 + r] = l;
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < rg.here * (D / 4); i += 64 * SPLIT) {
+        const int row = i / (D / 4), d = 4 * (i - row * (D / 4));
+        float jm = -INFINITY, jl = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < SPLIT; ++k) jm = fmaxf(jm, reinterpret_cast<const float*>(rings + k * Blk::RING)[16 * D + row]);
+        const float mz = jm == -INFINITY ? 0.0f : jm;
+#pragma unroll
+        for (int k = 0; k < SPLIT; ++k) {
+          const float* q = reinterpret_cast<const float*>(rings + k * Blk::RING);
+          const float w = __builtin_amdgcn_exp2f(q[16 * D + row] - mz);
+          const float4 x = *reinterpret_cast<const float4*>(q + row * D + d);
+          o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+          jl = fmaf(w, q[16 * D + 16 + row], jl);
+        }
+        const PaRow to_row(p, rg, b, kv, ROWS * group + row, jl);
+        to_row.write(d, o.x, o.y, o.z, o.w);
+        if (d == 0) to_row.write_lse(p, jm, jl);
+      }
+    } else if (r < rg.here) {
       if (whole) {
         const PaRow row(p, rg, b, kv, ROWS * group + r, l);
 #pragma unroll
@@ -762,9 +802,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
 
 // How a call is cut. waves: of a workgroup, each with 16 rows of the row group; they share one read of the keys (32 tokens of 16
 // heads, 8 sequences of 8000 keys of 64 values: 58 us, 97 with a wave a workgroup; 4 tokens of 8 heads a kv head, 16 sequences of
-// 25 000 keys of 128: 173 and 265). workgroups: 0, one an item, or the parts of a balanced line.
+// 25 000 keys of 128: 173 and 265). split: waves that share an item's blocks.
+// workgroups: 0, one an item, or the parts of a balanced line.
 struct PaPlan {
-  int64_t waves, groups, items, workgroups;
+  int64_t waves, split, groups, items, workgroups;
 };
 static PaPlan pa_plan(int64_t B, int64_t G, int64_t KV, int64_t T, int64_t D, bool f8, int64_t page, int64_t M,
                       int64_t window) {
@@ -775,8 +816,19 @@ static PaPlan pa_plan(int64_t B, int64_t G, int64_t KV, int64_t T, int64_t D, bo
   int64_t keys = M * page;
   if (window < keys) keys = window + T - 1 < keys ? window + T - 1 : keys;
   const int64_t items = c.items = B * c.groups * KV, held = (int64_t)pa_held((int)D, f8, (int)c.waves) * compute_units();
+  // Four waves an item, joined in LDS, where the ranges are short and the items leave room for the waves (their rings fit twice
+  // into a compute unit, bf16 of D = 128 once): 20 items of 256 keys of 64 6.4 us (balanced 9.1), 160 of 512 9.6 (12.1), 320 of
+  // 1024 20 (24), 480 of 256 10.0 (11.4, one wave an item). Not: 20 of 1024 12.8 (balanced 10.0), 8 of 512 of 128 12.7 (10.8),
+  // 800 of 256 16.7 (one wave 13.2), 512 of 120 of 128 16.1 (one wave 11.7).
+  const int64_t blocks = (keys + kPaKeys - 1) / kPaKeys, units = compute_units();
+  c.split = 1;
+  if (c.waves == 1 && blocks > 1 && items <= (D == 128 && !f8 ? 1 : 2) * units &&
+      (blocks <= 4 || (blocks <= 16 && blocks * units <= 32 * items))) {
+    c.split = 4;
+    return c;
+  }
   // One an item, and no second launch, where it pays or must be:
-  //   every item is a few blocks: 16 items of 100 keys 6.3 us, balanced 9.0; 20 of 256 8.7 and 9.1; but 160 of 512 15.9 and 12.0;
+  //   every item is a few blocks: 800 items of 256 keys 13.1 us; but 160 of 512 15.9, balanced 12.0;
   //   none is long and they are enough to fill the GPU: 1280 items of 2048 keys at most 103 us, balanced 111; of 1024 56 and 62;
   //   but of 100 to 4096 137 and 132;
   //   finding one's part of the line, which walks all sequences, would take long, or the line does not fit 31 bits.
@@ -792,15 +844,16 @@ static size_t pa_workspace(const PaPlan& c, int64_t D) {
 }
 
 template <int D, bool F8, bool WIDE>
-static const void* pa_kernel(int64_t waves) {
-  return waves == 1 ? reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 1>)
+static const void* pa_kernel(int64_t waves, int64_t split) {
+  return waves == 1 ? (split == 1 ? reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 1>)
+                                  : reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 1, 4>))
        : waves == 2 ? reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 2>)
                     : reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 4>);
 }
 template <int D>
-static const void* pa_kernel(bool f8, bool wide, int64_t waves) {
-  return f8 ? (wide ? pa_kernel<D, true, true>(waves) : pa_kernel<D, true, false>(waves))
-            : (wide ? pa_kernel<D, false, true>(waves) : pa_kernel<D, false, false>(waves));
+static const void* pa_kernel(bool f8, bool wide, int64_t waves, int64_t split) {
+  return f8 ? (wide ? pa_kernel<D, true, true>(waves, split) : pa_kernel<D, true, false>(waves, split))
+            : (wide ? pa_kernel<D, false, true>(waves, split) : pa_kernel<D, false, false>(waves, split));
 }
 template <int D>
 static const void* pa_join(int64_t waves) {
@@ -867,13 +920,13 @@ extern "C" int flw_paged_attention(const void* q, const int64_t* q_strides, cons
   p.by_g = by(H / KV); p.by_groups = by(c.groups); p.by_kv = by(KV);
   p.window = (int)w; p.balanced = c.workgroups != 0; p.scale = scale * 1.44269504088896341f;
   const bool f8 = cache_dtype == FLW_E4M3, wide = page_size >= kPaKeys;
-  const void* kern = D == 32 ? pa_kernel<32>(f8, wide, c.waves) : D == 64 ? pa_kernel<64>(f8, wide, c.waves)
-                                                                           : pa_kernel<128>(f8, wide, c.waves);
+  const void* kern = D == 32 ? pa_kernel<32>(f8, wide, c.waves, c.split) : D == 64 ? pa_kernel<64>(f8, wide, c.waves, c.split)
+                                                                           : pa_kernel<128>(f8, wide, c.waves, c.split);
   const void* join = D == 32 ? pa_join<32>(c.waves) : D == 64 ? pa_join<64>(c.waves) : pa_join<128>(c.waves);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Timer tm = take_timer();
   const dim3 grid((unsigned)(c.workgroups != 0 ? c.workgroups : items));
-  (void)launch_ext(kern, grid, dim3((unsigned)(64 * c.waves)), 0, s, p, tm.start, c.workgroups == 0 ? tm.stop : nullptr);
+  (void)launch_ext(kern, grid, dim3((unsigned)(64 * c.waves * c.split)), 0, s, p, tm.start, c.workgroups == 0 ? tm.stop : nullptr);
   if (c.workgroups != 0) {
     const int64_t rows = p.rows < 16 * c.waves ? p.rows : 16 * c.waves;
     (void)launch_ext(join, dim3((unsigned)items, (unsigned)((rows * (D / 4) + 31) / 32)), dim3(256), 0, s, p, nullptr,

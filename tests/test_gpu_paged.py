@@ -104,6 +104,11 @@ ATTENTION = [
     (1, 8, 8, 64, 32, "e4m3", [1500], None, 1000),
     (1, 6, 16, 32, 64, "bf16", [1200, 40], [16, 11], None),         # two groups of rows
     (1, 8, 16, 128, 128, "bf16", [1100], None, 600),
+    (4, 3, 1, 64, 64, "bf16", [256, 1, 0, 65, 129], None, None),    # four waves an item, some without a block
+    (2, 2, 4, 128, 32, "bf16", [200, 4, 90], [4, 4, 1], 70),
+    (2, 1, 2, 32, 16, "e4m3", [255, 2, 64], None, None),
+    (40, 1, 1, 64, 16, "e4m3", [500, 3, 130], None, None),
+    (70, 2, 1, 32, 64, "bf16", [900, 1000], None, None),
 ]
 
 
