@@ -491,8 +491,12 @@ struct RopeNode : torch::autograd::Function<RopeNode> {
     const int64_t how = ctx->saved_data["how"].toInt(), stream = ctx->saved_data["stream"].toInt();
     const bool two = how & 4, q = g[0].defined(), k = two && g[1].defined();
     if (!q && !k) return out;
-    const auto x = apply(q ? g[0] : g[1], q && k ? OptTensor(g[1]) : OptTensor(), saved[0], saved[1],
-                         saved[2].defined() ? OptTensor(saved[2]) : OptTensor(), (how & 1) != 0, (how & 2) == 0, stream);
+    const Tensor& first = q ? g[0] : g[1];
+    const bool half = (how & 1) != 0, inverse = (how & 2) == 0;
+    const auto x = c10::GradMode::is_enabled()            // a gradient of the gradient may be asked for
+                       ? apply(first, q && k ? OptTensor(g[1]) : OptTensor(), saved[0], saved[1],
+                               saved[2].defined() ? OptTensor(saved[2]) : OptTensor(), half, inverse, stream)
+                       : rope(first, q && k ? g[1] : Tensor(), saved[0], saved[1], saved[2], half, inverse, stream);
     if (q) out[0] = x[0];
     if (k) out[1] = x[q ? 1 : 0];
     return out;
