@@ -6,7 +6,7 @@
 // Each K and V byte in the window is read once, from its page, and nothing else is of that size: the bound is HBM. A K / V head
 // is shared by G query heads and by the T new tokens: their T G rows are the columns of MFMA tiles, 16 a wave.
 //
-// A workgroup of one, two or four waves (by its rows) takes blocks of 64 keys on its own. K and V of a block go from the pool
+// A workgroup of one to four waves (by its rows) takes blocks of 64 keys on its own. K and V of a block go from the pool
 // straight to LDS (whole 128-byte lines, non-temporal: a plain reader gets 6.2 TB/s on this card and a non-temporal one 6.9, but
 // half lines, which operands loaded to registers would be, lose by it), the next block's on their way while this one's are
 // multiplied. A single wave needs no barrier, only its own count of loads; several meet once a block.
@@ -133,10 +133,11 @@ __device__ __forceinline__ uint4 pa_widen(uint32_t lo, uint32_t hi) {
 //
 // V: rows of 64 keys (WIDE: a page holds at least 64), or, for pages of 16 and 32, the block's four runs of 16 keys one after
 // the other, so that one load stays within one page.
-// Workgroups that a compute unit holds, by the registers (at most 128 to 180 a lane) and by LDS (32 KB rings: four; a fifth was to
-// fit the 160 KB and did not, which made two rounds of the line: 168 us instead of 148).
+// Workgroups that a compute unit holds, by the registers (at most 128 to 180 a lane) and by LDS (32 KB rings: four). One too many
+// makes two rounds of the line: a fifth 32 KB ring, which was to fit the 160 KB and did not, 168 us instead of 148; a fourth
+// workgroup of three waves of e4m3, D = 128, 152 instead of 133.
 constexpr int pa_held(int D, bool f8, int waves) {
-  return waves == 1 ? (D == 128 && !f8 ? 4 : 8) : D == 128 && !f8 ? 2 : waves == 2 ? 4 : 3;
+  return waves == 1 ? (D == 128 && !f8 ? 4 : 8) : D == 128 && !f8 ? 2 : waves == 4 || (waves == 3 && D == 128) ? 3 : 4;
 }
 
 template <int D_, bool F8_, bool WIDE_, int WAVES>
@@ -242,7 +243,7 @@ struct PaWave {
   // K (V) of block kb, `head` bytes into its pages, to LDS at `to`: this wave's share of the loads.
   template <int J>
   __device__ __forceinline__ bool mine() const {          // load J of a tile is this wave's
-    return WAVES == 1 || wave == (Blk::NI <= WAVES ? J : J / (Blk::NI / WAVES));
+    return WAVES == 1 || wave == J / ((Blk::NI + WAVES - 1) / WAVES);
   }
   static __device__ __forceinline__ int page_of(PaPages pg, int c) {
     return c == 0 ? pg.id0 : c == 1 ? pg.id1 : c == 2 ? pg.id2 : pg.id3;
@@ -362,7 +363,7 @@ struct PaPart {
 
 // SPLIT > 1: that many waves a workgroup, each on its own as with WAVES = 1, share the blocks of one item and join in LDS.
 template <int D, bool F8, bool WIDE, int WAVES, int SPLIT = 1>
-__global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES == 4 ? (D == 128 && !F8 ? 2 : 3) : 2) void paged_attn_kernel(PagedAttn p) {
+__global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES >= 3 ? (D == 128 && !F8 ? 2 : 3) : 2) void paged_attn_kernel(PagedAttn p) {
   using Blk = PaBlock<D, F8, WIDE, WAVES>;
   constexpr int DT = Blk::DT, KS = Blk::KS, NI = Blk::NI, TILE = Blk::TILE, ROWS = 16 * WAVES;
   constexpr int BUFS = Blk::BUFS, AHEAD = WAVES > 1 ? 1 : BUFS;
@@ -802,7 +803,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
 
 // How a call is cut. waves: of a workgroup, each with 16 rows of the row group; they share one read of the keys (32 tokens of 16
 // heads, 8 sequences of 8000 keys of 64 values: 58 us, 97 with a wave a workgroup; 4 tokens of 8 heads a kv head, 16 sequences of
-// 25 000 keys of 128: 173 and 265). split: waves that share an item's blocks.
+// 25 000 keys of 128: 173 and 265; 48 rows on three waves 64 us, on four 77). split: waves that share an item's blocks.
 // workgroups: 0, one an item, or the parts of a balanced line.
 struct PaPlan {
   int64_t waves, split, groups, items, workgroups;
@@ -811,7 +812,7 @@ static PaPlan pa_plan(int64_t B, int64_t G, int64_t KV, int64_t T, int64_t D, bo
                       int64_t window) {
   PaPlan c{};
   const int64_t rows = T * G;
-  c.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  c.waves = rows <= 48 ? (rows + 15) / 16 : 4;
   c.groups = (rows + 16 * c.waves - 1) / (16 * c.waves);
   int64_t keys = M * page;
   if (window < keys) keys = window + T - 1 < keys ? window + T - 1 : keys;
@@ -848,6 +849,7 @@ static const void* pa_kernel(int64_t waves, int64_t split) {
   return waves == 1 ? (split == 1 ? reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 1>)
                                   : reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 1, 4>))
        : waves == 2 ? reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 2>)
+       : waves == 3 ? reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 3>)
                     : reinterpret_cast<const void*>(&paged_attn_kernel<D, F8, WIDE, 4>);
 }
 template <int D>
@@ -859,6 +861,7 @@ template <int D>
 static const void* pa_join(int64_t waves) {
   return waves == 1 ? reinterpret_cast<const void*>(&paged_join_kernel<D, 1>)
        : waves == 2 ? reinterpret_cast<const void*>(&paged_join_kernel<D, 2>)
+       : waves == 3 ? reinterpret_cast<const void*>(&paged_join_kernel<D, 3>)
                     : reinterpret_cast<const void*>(&paged_join_kernel<D, 4>);
 }
 

@@ -109,6 +109,9 @@ ATTENTION = [
     (2, 1, 2, 32, 16, "e4m3", [255, 2, 64], None, None),
     (40, 1, 1, 64, 16, "e4m3", [500, 3, 130], None, None),
     (70, 2, 1, 32, 64, "bf16", [900, 1000], None, None),
+    (1, 5, 8, 128, 64, "bf16", [3000, 8], [8, 3], None),            # three waves of rows
+    (2, 3, 16, 32, 16, "e4m3", [1800, 16], None, None),
+    (1, 9, 5, 64, 32, "e4m3", [1300, 40], None, 900),
 ]
 
 
