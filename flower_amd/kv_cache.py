@@ -78,7 +78,8 @@ class PagedKVCache:
 
     def reserve(self, counts) -> torch.Tensor:
         """Room for counts[s] (a tensor, a list, or one number for all) more tokens of each sequence, as ``reserve_pages``
-        grants it; returns ``counts`` as granted, 0 for a sequence that found no room and for one that wanted none."""
+        grants it; returns ``counts`` as granted, 0 for a sequence that found no room and for one that wanted none. The
+        tokens are then given to every layer together: no more than the T that its heads have room for."""
         *_, granted = reserve_pages(self.tables, self.lens, self.refs, self._ints(counts), self.page_size, window=self.window,
                                     out=(self.tables, self.lens, self.refs))
         return self.counts.copy_(granted)

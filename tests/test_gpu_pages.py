@@ -175,3 +175,26 @@ def test_one_layer_pools_and_a_side_stream():
     assert all(torch.equal(x, y) for x, y in zip(a, b))
     assert all(torch.equal(x, y) for x, y in zip(compact_pages(k, v, a[0], a[2]), c))
     assert torch.equal(k[0], k1) and torch.equal(v[0], v1)
+
+
+def test_reorder_of_very_many_places():
+    """More places than one grid dimension takes: forks into the first, the middle and the last ones."""
+    from flower_amd.kernels import reorder_pages
+    S, P = 40000, 12
+    k, v = pools(2, P, 1, 16, 32, torch.bfloat16)
+    wk, wv = k.clone(), v.clone()
+    tables, lens, refs, parents = torch.full((S, 1), -1, dtype=torch.int32), torch.zeros(S, dtype=torch.int32), \
+        torch.zeros(P, dtype=torch.int32), torch.arange(S, dtype=torch.int32)
+    for s in range(3):                       # places 0, 1, 2 hold pages 3, 4, 5 and 5 + s positions
+        tables[s], lens[s], refs[3 + s] = 3 + s, 5 + s, 1
+    forks = [(5, 2), (32767, 0), (32768, 1), (32769, 2), (39999, 0)]
+    for place, parent in forks:
+        parents[place] = parent
+    t, n, r = (x.cuda() for x in (tables, lens, refs))
+    t, n, r = reorder_pages(k, v, t, n, r, parents.cuda(), out=(t, n, r))
+    for (place, parent), page in zip(forks, (0, 1, 2, 6, 7)):        # the free pages in the order of the places
+        tables[place], lens[place], refs[page] = page, 5 + parent, 1
+        wk[:, page, :, :5 + parent] = wk[:, 3 + parent, :, :5 + parent]
+        wv[:, page, :, :, :5 + parent] = wv[:, 3 + parent, :, :, :5 + parent]
+    assert torch.equal(t.cpu(), tables) and torch.equal(n.cpu(), lens) and torch.equal(r.cpu(), refs)
+    assert torch.equal(k, wk) and torch.equal(v, wv)
