@@ -11,7 +11,8 @@
 
 #include "flw_common.h"
 
-// m0 is clobbered by the direct-to-LDS loads below; nothing else here uses it.
+// m0 is clobbered by the direct-to-LDS loads below; nothing else here uses it. Between its write and the load stands the wait
+// state that the hardware asks for, which the compiler does not put inside an assembly statement.
 #pragma clang diagnostic ignored "-Winline-asm"
 
 namespace flw {
@@ -461,7 +462,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, uint8_t* st0, uin
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8_t*)(stage + lbase);
 #pragma unroll
     for (int t = 0; t < 8; ++t)
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :: "s"(lds + t * 1024), "v"(goff[t] + k0 - (((hi_half >> t) & 1u) ? back : 0u)), "s"(gsrc)
                    : "memory", "m0");
   };
@@ -622,7 +623,7 @@ __device__ __forceinline__ void gemm_tile_128(const GemmParams& p, uint8_t* st0,
       const bool xop = row0 >= 256;
       const uint32_t dst = lds + (xop ? kFOpBytes + (row0 - 256) * 128 : row0 * 128);
       const uint8_t* src = xop ? p.x8 : p.w8;
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :: "s"(dst), "v"(goff[t] + k0 - (((hi_half >> t) & 1u) ? back : 0u)), "s"(src)
                    : "memory", "m0");
     }
@@ -1008,7 +1009,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_gemm_ring_kernel(GemmParams 
     for (int q = 0; q < IPW; ++q) {
       const int row0 = 8 * (wave * IPW + q);
       const uint8_t* src = row0 >= BN ? x8 : w8;
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :: "s"(dst + row0 * 128), "v"(goff[q] + (uint32_t)s * kFBK - (((hi_half >> q) & 1u) ? back : 0u)),
                       "s"(src) : "memory", "m0");
     }
@@ -1216,11 +1217,11 @@ __device__ __forceinline__ void w8a16_tile(const W8A16Params& p, uint8_t* lds, i
     const uint32_t lw = (uint32_t)(uintptr_t)(lds_u8_t*)(stage + kWXBytes + 32 * wave * 64);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :: "s"(lx + t * 1024), "v"(xoff[t] + kx), "s"(p.x) : "memory", "m0");
 #pragma unroll
     for (int t = 0; t < 2; ++t)
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :: "s"(lw + t * 1024), "v"(woff[t] + kw), "s"(p.w8) : "memory", "m0");
   };
 
@@ -1381,10 +1382,10 @@ __global__ __launch_bounds__(64 * WN * WM) void w8a16_ring_kernel(W8A16Params p)
       for (int q = 0; q < IPW; ++q) {
         const int ins = wave * IPW + q;
         if (ins < kXIns)
-          asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                        :: "s"(dst + ins * 1024), "v"(off[q] + (uint32_t)s * (kWK * 2)), "s"(x) : "memory", "m0");
         else
-          asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                        :: "s"(dst + ins * 1024), "v"(off[q] + (uint32_t)s * kWK), "s"(w8) : "memory", "m0");
       }
     };

@@ -169,15 +169,17 @@ struct PaBlock {
 
 // 64 lanes' 16 bytes from sbase + voff to LDS at lds + OFF, in lane order, non-temporal (5 to 15 % faster where keys are read once,
 // 7 % slower where eight row groups read them). Issued from inline assembly: the
-// compiler then does not drain the loads before every read of LDS; the kernel waits for them itself, by count.
+// compiler then does not drain the loads before every read of LDS; the kernel waits for them itself, by count. A load to LDS that
+// follows the write of M0 at once may go by M0's old value: one wait state, which the compiler does not put inside the statement.
 template <int OFF>
 __device__ __forceinline__ void pa_dma(uint32_t lds, uint32_t voff, const uint8_t* sbase) {
-  asm volatile("s_add_u32 m0, %0, %3\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(voff), "s"(sbase), "n"(OFF)
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(voff), "s"(sbase), "n"(OFF)
                  : "memory", "m0", "scc");
 }
 template <int OFF>
 __device__ __forceinline__ void pa_dma_lanes(uint32_t lds, const uint8_t* a) {       // each lane its own address
-  asm volatile("s_add_u32 m0, %0, %2\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(a), "n"(OFF) : "memory", "m0", "scc");
+  asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(a), "n"(OFF)
+                 : "memory", "m0", "scc");
 }
 // The results of a run of MFMAs, safe to read from here on whichever way the code goes: the compiler counts the cycles between
 // an MFMA and the first reader of its result only along the fall-through path, so that a branch in between, taken, reached the

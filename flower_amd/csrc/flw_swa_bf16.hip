@@ -130,7 +130,7 @@ struct TileLoadLds {
 #pragma unroll
     for (int t = 0; t < NI; ++t) {
       const uint32_t dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(lds + RPI * (NI * wave + t) * 2 * D);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    :: "s"(dst), "v"(off[t] + (uint32_t)row0 * row_bytes), "s"(rs) : "memory", "m0");
     }
   }
