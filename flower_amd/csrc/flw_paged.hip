@@ -509,13 +509,21 @@ __global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES >= 3 ? (D == 128 && !F8 ?
     for (int dt = 0; dt < DT; ++dt) acc[dt] = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
     float c = p.scale;
     if (p.k_scale != nullptr) c *= p.k_scale[kv];
-    if (c < 0.0f) {                                       // a negative scale goes to q, so that larger scores weigh more
-      c = -c;
+    if (c <= 0.0f) {
+      // A negative scale goes to q, so that larger scores weigh more. A scale of zero does, too: a masked score is -infinity, and
+      // zero times that is no weight. Zero times q is NaN where q is not finite, as times a key, which the product sees to.
+      const bool zero = c == 0.0f;
+      c = zero ? 1.0f : -c;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        uint4 w = __builtin_bit_cast(uint4, qf[k]);
-        w = make_uint4(w.x ^ 0x80008000u, w.y ^ 0x80008000u, w.z ^ 0x80008000u, w.w ^ 0x80008000u);
-        qf[k] = __builtin_bit_cast(pa_bf8, w);
+        const uint4 w = __builtin_bit_cast(uint4, qf[k]);
+        uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo = (x[e] & 0x7F80u) == 0x7F80u ? 0x7FC0u : 0u, hi = (x[e] >> 16 & 0x7F80u) == 0x7F80u ? 0x7FC0u : 0u;
+          x[e] = zero ? lo | hi << 16 : x[e] ^ 0x80008000u;
+        }
+        qf[k] = __builtin_bit_cast(pa_bf8, make_uint4(x[0], x[1], x[2], x[3]));
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // q, and what the part before wrote: only blocks are counted below
