@@ -224,7 +224,7 @@ def rotary_tables(rotary_dim: int, positions: int, base: float = 10000.0, scalin
         def pair(turns: float) -> float:                 # the (fractional) pair that turns so often in `length` positions
             return rotary_dim * math.log(length / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
 
-        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rotary_dim // 2 - 1)
+        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rotary_dim - 1)
         slower = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
         freq = freq * (1.0 - slower) + freq / factor * slower
     if scaling:
