@@ -7,6 +7,7 @@
 // cache's operators are here as a whole, their checks and the one's autograd node too: their kernels
 // take 3 to 6 us in a decode step, less than the same checks take in Python.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -419,6 +420,13 @@ void check_ints(const char* name, const Tensor& t, at::IntArrayRef sizes, const 
                 " on ", t.device());
 }
 
+// A derivative of t is asked for in reverse mode (backward); in forward mode, which no operator here has: none is dropped.
+bool wants_backward(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+void refuse_tangent(const char* what, const Tensor& t) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    throw std::runtime_error(text(what, " has no forward-mode derivative: call it on tensors without a tangent"));
+}
+
 int32_t* i32(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 int32_t* i32(const OptTensor& t) { return t ? i32(*t) : nullptr; }
 float* f32(const OptTensor& t) { return t ? f32(*t) : nullptr; }
@@ -447,8 +455,9 @@ void check_rotary_tables(const Tensor& cos, const Tensor& sin, const Tensor& q) 
   REFUSE_UNLESS(R > 0 && R <= q.size(3) && R % 8 == 0, "rotary_dim must be a multiple of 8 up to the head_dim ", q.size(3),
                 ", got ", R);
   REFUSE_UNLESS(cos.device() == q.device() && sin.device() == q.device(), "cos and sin must be on ", q.device());
-  REFUSE_UNLESS(!(c10::GradMode::is_enabled() && (cos.requires_grad() || sin.requires_grad())),
-                "the rotary tables take no gradient");
+  REFUSE_UNLESS(!wants_backward(cos) && !wants_backward(sin), "the rotary tables take no gradient");
+  refuse_tangent("a rotary table", cos);
+  refuse_tangent("a rotary table", sin);
 }
 
 // q, k (undefined: none) turned, contiguous: (q') or (q', k').
@@ -491,6 +500,8 @@ struct RopeNode : torch::autograd::Function<RopeNode> {
     const int64_t how = ctx->saved_data["how"].toInt(), stream = ctx->saved_data["stream"].toInt();
     const bool two = how & 4, q = g[0].defined(), k = two && g[1].defined();
     if (!q && !k) return out;
+    for (const Tensor& t : g)
+      if (t.defined()) refuse_tangent("apply_rotary's gradient", t);
     const Tensor& first = q ? g[0] : g[1];
     const bool half = (how & 1) != 0, inverse = (how & 2) == 0;
     const auto x = c10::GradMode::is_enabled()            // a gradient of the gradient may be asked for
@@ -524,8 +535,10 @@ std::tuple<Tensor, OptTensor> apply_rotary(const Tensor& q, const OptTensor& k, 
     REFUSE_UNLESS(pos.device() == q.device(), "positions must be on ", q.device());
     if (T > 1 && pos.stride(-1) != 1) at = pos.contiguous();
   }
+  refuse_tangent("apply_rotary", q);
+  if (k) refuse_tangent("apply_rotary", *k);
   require_gpu(q);
-  const bool grad = c10::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()));
+  const bool grad = wants_backward(q) || (k && wants_backward(*k));
   const auto x = grad ? RopeNode::apply(q, k, cos, sin, at, half, false, stream)
                       : rope(q, k.value_or(Tensor()), cos, sin, at.value_or(Tensor()), half, false, stream);
   return {x[0], k ? OptTensor(x[1]) : OptTensor()};
@@ -556,6 +569,11 @@ void check_scales(const Tensor& k_pages, const OptTensor& k_scale, const OptTens
                   "an e4m3 cache needs ", t == &k_scale ? "k_scale" : "v_scale", ", contiguous float32 (", k_pages.size(1), ",) on ",
                   k_pages.device());
 }
+void refuse_gradients(const char* what, const Tensor& t) {
+  if (wants_backward(t))
+    throw std::runtime_error(text(what, " is forward-only: call it under torch.no_grad() or on detached tensors"));
+  refuse_tangent(what, t);
+}
 void check_tokens(const char* what, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,
                   const Tensor& lens, const OptTensor& counts, const OptTensor& k_scale, const OptTensor& v_scale) {
   check_pool(k_pages, v_pages, 4);
@@ -572,8 +590,9 @@ void check_tokens(const char* what, const Tensor& q, const Tensor& k_pages, cons
   check_ints("lens", lens, {q.size(0)}, q);
   if (counts) check_ints("counts", *counts, {q.size(0)}, q);
   check_scales(k_pages, k_scale, v_scale);
-  if (c10::GradMode::is_enabled() && q.requires_grad())
-    throw std::runtime_error(text(what, " is forward-only: call it under torch.no_grad() or on detached tensors"));
+  for (const Tensor* t : {&q, &k_pages, &v_pages}) refuse_gradients(what, *t);
+  for (const OptTensor* t : {&k_scale, &v_scale})
+    if (*t) refuse_gradients(what, **t);
 }
 
 std::tuple<Tensor, OptTensor> paged_append(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& k_pages,
@@ -587,8 +606,7 @@ std::tuple<Tensor, OptTensor> paged_append(const Tensor& q0, const Tensor& k0, c
                       t->size(3) == q0.size(3) && t->scalar_type() == q0.scalar_type() && t->device() == q0.device(),
                   "k and v must be (", q0.size(0), ", ", k_pages.size(1), ", ", q0.size(2), ", ", q0.size(3), ") as q, got ",
                   t->sizes(), " ", t->scalar_type());
-    if (c10::GradMode::is_enabled() && t->requires_grad())
-      throw std::runtime_error("paged_append is forward-only: call it under torch.no_grad() or on detached tensors");
+    refuse_gradients("paged_append", *t);
   }
   REFUSE_UNLESS(cos.has_value() == sin.has_value(), "give both cos and sin, or neither");
   if (cos) check_rotary_tables(*cos, *sin, q0);

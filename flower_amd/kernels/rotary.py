@@ -23,7 +23,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin
     The first R = 2 * cos.shape[1] values of each head are pairs (a, b), (2 i, 2 i + 1) ("interleaved") or (i, i + R / 2)
     ("half"), and become (a c - b s, b c + a s) with c = cos[position, i], s = sin[position, i]; the rest of the head is
     copied. cos, sin: fp32 [positions, R / 2]. positions: int32 or int64 (T,) or (B, T); None is 0 .. T - 1. A position
-    outside the tables makes that token's pairs NaN. fp32 arithmetic, rounded once to q's dtype. Differentiable in q and k.
+    outside the tables makes that token's pairs NaN. fp32 arithmetic, rounded once to q's dtype. Differentiable in q
+    and k by backward, also twice; tensors with a forward-mode tangent are refused.
     """
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
