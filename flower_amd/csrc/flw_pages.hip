@@ -25,6 +25,7 @@ struct PagesParams {
   int32_t* lens_out;
   int32_t* refs_out;
   int32_t* granted;               // reserve
+  int32_t* kept;                  // reorder, or NULL: 1 where place s holds what stood at its parent, 0 where it is empty instead
   int32_t* need;                  // workspace: [S] pages wanted, -1 where the request cannot be met at all
   int32_t* pairs;                 // workspace: [S][3] dst, src, tokens to copy (dst -1: nothing)
   int32_t* list;                  // workspace: [P] free pages in ascending order
@@ -221,6 +222,7 @@ __global__ __launch_bounds__(256) void reorder_rows_kernel(PagesParams p) {
     p.pairs[3 * s + 1] = copies ? src : -1;
     p.pairs[3 * s + 2] = used;
     p.lens_out[s] = len;
+    if (p.kept != nullptr) p.kept[s] = real;
   }
 }
 
@@ -256,6 +258,7 @@ __global__ __launch_bounds__(kScan) void reorder_take_kernel(PagesParams p) {
         row[j] = -1;
       }
       p.lens_out[s] = 0;
+      if (p.kept != nullptr) p.kept[s] = 0;
     }
   }
 }
@@ -469,6 +472,15 @@ extern "C" int flw_reorder_pages(void* k_pages, void* v_pages, int cache_dtype, 
                                  const int32_t* refs, const int32_t* parents, int64_t S, int64_t table_cols,
                                  int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, void* workspace,
                                  size_t workspace_bytes, void* stream) {
+  return flw_reorder_pages_kept(k_pages, v_pages, cache_dtype, L, num_pages, KV, page_size, D, tables, lens, refs, parents, S,
+                                table_cols, tables_out, lens_out, refs_out, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int flw_reorder_pages_kept(void* k_pages, void* v_pages, int cache_dtype, int64_t L, int64_t num_pages, int64_t KV,
+                                      int64_t page_size, int64_t D, const int32_t* tables, const int32_t* lens,
+                                      const int32_t* refs, const int32_t* parents, int64_t S, int64_t table_cols,
+                                      int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int32_t* kept,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
   int rc = pages_check(tables, lens, refs, S, table_cols, num_pages);
   if (rc || (rc = page_size_check(page_size)) != 0 || (rc = pool_check(k_pages, v_pages, L, KV, D, cache_dtype)) != 0) return rc;
   FLW_REQUIRE(parents && tables_out && lens_out && refs_out, FLW_E_INVALID, "null pointer");
@@ -484,7 +496,7 @@ extern "C" int flw_reorder_pages(void* k_pages, void* v_pages, int cache_dtype, 
   // a place's row is written while its children still read it: in place, they read a copy
   const bool in_place = tables_out == tables, lens_in_place = lens_out == lens;
   p.tables = in_place ? tables_ws : tables; p.lens = lens_in_place ? lens_ws : lens; p.refs = refs; p.arg = parents;
-  p.tables_out = tables_out; p.lens_out = lens_out; p.refs_out = refs_out;
+  p.tables_out = tables_out; p.lens_out = lens_out; p.refs_out = refs_out; p.kept = kept;
   p.S = (int)S; p.M = (int)table_cols; p.P = (int)num_pages; p.shift = __builtin_ctzll(page_size);
   hipStream_t s = static_cast<hipStream_t>(stream);
   copy_ints(CopyInts{{refs_out, in_place ? tables_ws : nullptr, lens_in_place ? lens_ws : nullptr},

@@ -710,9 +710,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> reserve_pages(const Tensor& tables, c
   return {to[0], to[1], to[2], granted};
 }
 
-std::tuple<Tensor, Tensor, Tensor> reorder_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,
-                                                 const Tensor& lens, const Tensor& refs, const Tensor& parents,
-                                                 const OutTensors& out, int64_t stream) {
+std::tuple<Tensor, Tensor, Tensor, OptTensor> reorder_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,
+                                                            const Tensor& lens, const Tensor& refs, const Tensor& parents,
+                                                            const OutTensors& out, bool with_kept, int64_t stream) {
   check_state(tables, refs);
   const int64_t S = tables.size(0), M = tables.size(1), P = refs.size(0);
   check_ints("lens", lens, {S}, tables);
@@ -722,11 +722,13 @@ std::tuple<Tensor, Tensor, Tensor> reorder_pages(const Tensor& k_pages, const Te
   const std::vector<Tensor> to = outputs(out, {tables, lens, refs}, parents);
   c10::DeviceGuard guard(tables.device());
   Tensor ws = workspace(lens, flw_reorder_pages_workspace_bytes(S, M, P));
-  check(flw_reorder_pages(k.data_ptr(), v.data_ptr(), cache_code(k), k.size(0), P, k.size(2), k.size(3), k.size(4), i32(tables),
-                          i32(lens), i32(refs), i32(parents), S, M, i32(to[0]), i32(to[1]), i32(to[2]), ws.data_ptr(),
-                          (size_t)ws.numel(), str(stream)),
+  OptTensor kept;
+  if (with_kept) kept = empty(lens, {S}, at::kInt);
+  check(flw_reorder_pages_kept(k.data_ptr(), v.data_ptr(), cache_code(k), k.size(0), P, k.size(2), k.size(3), k.size(4),
+                               i32(tables), i32(lens), i32(refs), i32(parents), S, M, i32(to[0]), i32(to[1]), i32(to[2]),
+                               i32(kept), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
         "reorder_pages");
-  return {to[0], to[1], to[2]};
+  return {to[0], to[1], to[2], kept};
 }
 
 std::tuple<Tensor, Tensor, Tensor> compact_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,

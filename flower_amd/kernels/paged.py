@@ -78,7 +78,7 @@ def reserve_pages(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, 
 
 
 def reorder_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor,
-                  parents: torch.Tensor, *, out=None):
+                  parents: torch.Tensor, *, out=None, return_kept: bool = False):
     """(tables, lens, refs), with place s holding a copy of the sequence that stood at parents[s] (int32): itself stays, any
     other forks it, a number that is no place (-1) leaves s empty and its pages to whoever else holds them.
 
@@ -86,8 +86,12 @@ def reorder_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Te
     first), each other child gets a free page (the lowest numbers first, in the order of s) and a copy of its positions, in
     the pools of all layers: k_pages (layers, pages, ..), v_pages, or one layer's. A place whose page cannot be had is
     emptied: its lens is 0. Pages that nobody holds any more can be taken in the same call. out: as in ``reserve_pages``.
+    ``return_kept`` adds kept (S,) int32: 1 where place s holds its copy (an empty sequence's, too), 0 where it was to be
+    emptied or is for want of a page.
     """
-    return _lib.native().reorder_pages(k_pages, v_pages, tables, lens, refs, parents, out, _lib.stream_or_none(tables))
+    *state, kept = _lib.native().reorder_pages(k_pages, v_pages, tables, lens, refs, parents, out, return_kept,
+                                               _lib.stream_or_none(tables))
+    return (*state, kept) if return_kept else tuple(state)
 
 
 def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, refs: torch.Tensor, *, out=None):

@@ -97,12 +97,15 @@ class PagedKVCache:
         return paged_attention(q, self.k_pages[layer], self.v_pages[layer], self.tables, self.lens, self.counts, window=window,
                                **self._scales(layer), **how)
 
-    def reorder(self, parents) -> None:
-        """Place s becomes a copy of the sequence at parents[s], or empty (-1), as ``reorder_pages`` does. ``counts`` is then
+    def reorder(self, parents) -> torch.Tensor:
+        """Place s becomes a copy of the sequence at parents[s], or empty (-1), as ``reorder_pages`` does; returns its kept (S,)
+        int32, on the GPU: 0 for a place that was to be emptied, and for one whose copy found no page and that is empty, too.
+        Such a place must not go on as its parent: ``reserve(kept)`` gives one more token to the others only. ``counts`` is then
         of no sequence: ``reserve`` comes next."""
-        reorder_pages(self.k_pages, self.v_pages, self.tables, self.lens, self.refs, self._ints(parents),
-                      out=(self.tables, self.lens, self.refs))
+        *_, kept = reorder_pages(self.k_pages, self.v_pages, self.tables, self.lens, self.refs, self._ints(parents),
+                                 out=(self.tables, self.lens, self.refs), return_kept=True)
         self.counts.zero_()
+        return kept
 
     def free(self, places) -> None:
         """Empties the given places (numbers); their pages can be taken again where no fork holds them."""
