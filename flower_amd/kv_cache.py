@@ -23,7 +23,8 @@ class PagedKVCache:
     window / page_size and two more beside those of the tokens of one ``reserve``.
 
     ``tables`` (sequences, entries), ``lens`` (sequences,), ``refs`` (num_pages,) and ``counts`` (sequences,) int32 are the
-    state: counts are the tokens that the last ``reserve`` granted, which ``append`` and ``attend`` work on.
+    state: counts are the tokens that the last ``reserve`` granted (less those taken back), which ``append`` and ``attend``
+    work on.
     """
 
     def __init__(self, layers: int, num_pages: int, kv_heads: int, head_dim: int, *, sequences: int, max_len: int,
@@ -83,6 +84,18 @@ class PagedKVCache:
         *_, granted = reserve_pages(self.tables, self.lens, self.refs, self._ints(counts), self.page_size, window=self.window,
                                     out=(self.tables, self.lens, self.refs))
         return self.counts.copy_(granted)
+
+    def take_back(self, counts) -> None:
+        """The last counts[s] (as ``reserve`` takes them) of the tokens that the last ``reserve`` granted are no more: drafted
+        tokens that were not accepted. No more than were granted, so that a sequence never becomes shorter than a fork of it
+        was, whose full pages it shares, nor than its window needs: lower ``lens`` by this alone. The pages stay with the
+        sequence for its next tokens."""
+        counts = self._ints(counts)
+        if counts.shape != self.counts.shape:
+            raise ValueError(f"counts must be ({self.sequences},), got {tuple(counts.shape)}")
+        counts = torch.minimum(counts.clamp(min=0), self.counts)
+        self.lens.sub_(counts)
+        self.counts.sub_(counts)
 
     def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, **how):
         """``paged_append`` of the reserved tokens' heads to a layer's pool (``how``: its rotary and norm arguments)."""
