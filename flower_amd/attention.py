@@ -262,8 +262,7 @@ class RotaryEmbedding(nn.Module):
         cos, sin = self._tables(max_seq_len) if self.plain else (None, None)
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
-        self._cast = {}
-        self._pairs = {}
+        self._made, self._last = {}, {}                  # what _kept made: all of it, and its last answers
         if not self.plain:
             rotary_tables(rotary_dim, 1, base, scaling)  # refuses what it cannot scale
 
@@ -279,7 +278,27 @@ class RotaryEmbedding(nn.Module):
         cos, sin = self._tables(seq_len)
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
-        self._cast = {}
+
+    def _kept(self, kind: str, seq_len: int, dtype, device, make):
+        """The first seq_len rows of the tables of ``kind``, made by make(rows) where there are none so long. What was handed out
+        stays where it is as long as the module lives: a captured graph reads it there on every replay. Longer tables come
+        besides, at least twice as long as the last ones, so that few do. Never inference tensors: training saves them."""
+        key = kind, dtype, torch.device(device)
+        last = self._last.get(key)
+        if last is not None and last[0] == seq_len and last[1] is self.cos:
+            return last[2]
+        made = [t for source, t in self._made.setdefault(key, []) if source is self.cos]
+        tables = next((t for t in made if t[0].shape[0] >= seq_len), None)
+        with torch.inference_mode(False), torch.no_grad():
+            if tables is None:
+                rows = max([seq_len] + [2 * t[0].shape[0] for t in made])
+                if self.plain and seq_len > self.cos.shape[-2]:
+                    self._extend_cache(rows)
+                tables = make(rows if not self.plain else min(rows, self.cos.shape[-2]))
+                self._made[key].append((self.cos, tables))
+            views = tuple(t[:seq_len] for t in tables)
+        self._last[key] = seq_len, self.cos, views
+        return views
 
     @staticmethod
     def _rotate_half(x: torch.Tensor) -> torch.Tensor:
@@ -291,32 +310,17 @@ class RotaryEmbedding(nn.Module):
         """(cos, sin) as contiguous [seq_len, head_dim] tensors of ``dtype`` on ``device``."""
         if not self.plain:
             raise ValueError("tables of whole interleaved heads are for plain RoPE: use pair_tables")
-        if seq_len > self.cos.shape[-2]:
-            self._extend_cache(seq_len)
-        key = (seq_len, dtype, torch.device(device), self.cos.data_ptr())
-        hit = self._cast.get(key)
-        if hit is None:
-            hit = tuple(t[0, 0, :seq_len].to(device=device, dtype=dtype).contiguous() for t in (self.cos, self.sin))
-            self._cast = {key: hit}
-        return hit
+        return self._kept("whole", seq_len, dtype, device, lambda rows: tuple(
+            t[0, 0, :rows].to(device=device, dtype=dtype).contiguous() for t in (self.cos, self.sin)))
 
     def pair_tables(self, seq_len: int, dtype: torch.dtype, device) -> tuple[torch.Tensor, torch.Tensor]:
         """(cos, sin) fp32 [seq_len, rotary_dim / 2] for ``apply_rotary`` and ``paged_append``: the values that ``forward``
         multiplies heads of ``dtype`` by (plain: rounded to it)."""
         if not self.plain:                               # fp32 whatever the module is cast to
-            hit = self._pairs.get(torch.device(device))
-            if hit is None or hit[0].shape[0] < seq_len:
-                hit = rotary_tables(self.rotary_dim, max(seq_len, self._max_seq_len), self._base, self._scaling, device)
-                self._pairs = {torch.device(device): hit}
-            return hit[0][:seq_len], hit[1][:seq_len]
-        if seq_len > self.cos.shape[-2]:
-            self._extend_cache(seq_len)
-        key = (seq_len, dtype, torch.device(device), self.cos.data_ptr())
-        hit = self._pairs.get(key)
-        if hit is None:
-            hit = tuple(t[0, 0, :seq_len, ::2].to(device=device, dtype=dtype).float().contiguous() for t in (self.cos, self.sin))
-            self._pairs = {key: hit}
-        return hit
+            return self._kept("pairs", seq_len, torch.float32, device,
+                              lambda rows: rotary_tables(self.rotary_dim, rows, self._base, self._scaling, device))
+        return self._kept("pairs", seq_len, dtype, device, lambda rows: tuple(
+            t[0, 0, :rows, ::2].to(device=device, dtype=dtype).float().contiguous() for t in (self.cos, self.sin)))
 
     def forward(self, q: torch.Tensor, k: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         if not self.plain:
