@@ -75,7 +75,12 @@ class PagedKVCache:
     def _ints(self, values) -> torch.Tensor:
         if isinstance(values, int):
             return torch.full((self.sequences,), values, dtype=torch.int32, device=self.lens.device)
-        return torch.as_tensor(values, dtype=torch.int32, device=self.lens.device).contiguous()
+        values = torch.as_tensor(values)
+        if values.is_floating_point() or values.is_complex():
+            raise TypeError(f"counts and places are whole numbers, got {values.dtype}")
+        if values.dtype == torch.int64:                  # beyond 32 bits: as far as those go, not what is left of it
+            values = values.clamp(-2 ** 31, 2 ** 31 - 1)
+        return values.to(device=self.lens.device, dtype=torch.int32).contiguous()
 
     def reserve(self, counts) -> torch.Tensor:
         """Room for counts[s] (a tensor, a list, or one number for all) more tokens of each sequence, as ``reserve_pages``

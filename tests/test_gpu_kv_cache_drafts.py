@@ -110,3 +110,13 @@ def test_a_captured_draft_and_its_taking_back():
         assert torch.equal(out, want) and bool(torch.isfinite(out).all()), n
         assert all(torch.equal(getattr(cache, a), getattr(twin, a)) for a in ("tables", "lens", "refs", "counts")), n
     assert cache.lens.tolist() == [24, 9, 12]
+
+
+def test_whole_numbers_beyond_32_bits_are_not_cut():
+    cache = make(torch.bfloat16, None)
+    far = torch.tensor([2 ** 32 + 1, 2 ** 31, -2 ** 32 + 3], device="cuda")
+    for counts in (far, far.tolist(), far.cpu().numpy()):
+        assert cache.reserve(counts).tolist() == [0, 0, 0] and cache.lens.tolist() == [0, 0, 0]
+    cache.reserve([3, 2, 1])
+    assert cache.reorder(torch.tensor([2 ** 32, 1, -2 ** 32 + 2], device="cuda")).tolist() == [0, 1, 0]
+    assert cache.lens.tolist() == [0, 2, 0]
