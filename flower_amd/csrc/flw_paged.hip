@@ -25,9 +25,12 @@
 // and cut into equal parts, one for each workgroup that the GPU holds; an item cut by a border leaves fp32 partial results, which
 // a second launch joins. A workgroup begins an item's loads while it ends the one before.
 //
-// Measured: 64 sequences of up to 2048 keys, 20 heads of 64: 103 us, 5.9 TB/s of K and V. 4 sequences of 70 001 to 131 072 keys, 32
-// heads on 4 of 128: 138 us, 5.9 TB/s. Short calls are latency: 100 keys of 16 heads take 5.9 us, most of it the first fetch of
-// the code and of the page numbers, the lengths and the keys that depend on each other.
+// Measured: 64 sequences of up to 2048 keys, 20 heads of 64: 99 us, 6.1 TB/s of K and V. 4 sequences of 70 001 to 131 072 keys, 32
+// heads on 4 of 128: 133 us with the join, 6.2 TB/s. Short calls are latency: 100 keys of 16 heads take 5.8 us, most of it the
+// first fetch of the code and of the page numbers, the lengths and the keys that depend on each other.
+//
+// Keys and values that are not finite reach only the rows that see them; an infinite V may come out as NaN there, since the second
+// term of its weight is often zero or of the other sign.
 
 #include <utility>
 
@@ -123,6 +126,13 @@ __device__ __forceinline__ uint4 pa_widen(uint32_t lo, uint32_t hi) {
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, true)));
 }
 
+// Workgroups that a compute unit holds, by the registers (at most 128 to 180 a lane) and by LDS (32 KB rings: four). One too many
+// makes two rounds of the line: a fifth 32 KB ring, which was to fit the 160 KB and did not, 168 us instead of 148; a fourth
+// workgroup of three waves of e4m3, D = 128, 152 instead of 133.
+constexpr int pa_held(int D, bool f8, int waves) {
+  return waves == 1 ? (D == 128 && !f8 ? 4 : 8) : D == 128 && !f8 ? 2 : waves == 4 || (waves == 3 && D == 128) ? 3 : 4;
+}
+
 // The geometry of a block of 64 keys, K and V alike 64 D values: how its 16-byte chunks lie in LDS, and which lane of which
 // 1 KB load brings them. A load takes 64 chunks to consecutive places; a chunk's place within its row is its number xor a
 // function of the row (kswz, vswz), so that the 16 lanes that read one operand together meet 16 different bank groups.
@@ -133,13 +143,6 @@ __device__ __forceinline__ uint4 pa_widen(uint32_t lo, uint32_t hi) {
 //
 // V: rows of 64 keys (WIDE: a page holds at least 64), or, for pages of 16 and 32, the block's four runs of 16 keys one after
 // the other, so that one load stays within one page.
-// Workgroups that a compute unit holds, by the registers (at most 128 to 180 a lane) and by LDS (32 KB rings: four). One too many
-// makes two rounds of the line: a fifth 32 KB ring, which was to fit the 160 KB and did not, 168 us instead of 148; a fourth
-// workgroup of three waves of e4m3, D = 128, 152 instead of 133.
-constexpr int pa_held(int D, bool f8, int waves) {
-  return waves == 1 ? (D == 128 && !f8 ? 4 : 8) : D == 128 && !f8 ? 2 : waves == 4 || (waves == 3 && D == 128) ? 3 : 4;
-}
-
 template <int D_, bool F8_, bool WIDE_, int WAVES>
 struct PaBlock {
   static constexpr int D = D_;
@@ -181,9 +184,11 @@ __device__ __forceinline__ void pa_dma_lanes(uint32_t lds, const uint8_t* a) {  
   asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(a), "n"(OFF)
                  : "memory", "m0", "scc");
 }
-// The results of a run of MFMAs, safe to read from here on whichever way the code goes: the compiler counts the cycles between
-// an MFMA and the first reader of its result only along the fall-through path, so that a branch in between, taken, reached the
-// reader too early (the two last words of a result were seen stale).
+// The results of a run of MFMAs, safe to read from here on whichever way the code goes. In a form of this kernel with branches
+// inside its runs, results were seen stale, and the compiler's code was: two MFMAs into v[82:85]; s_cbranch_vccnz L; two MFMAs into
+// other registers and their readers; L: v_cndmask of v85. The taken way had no wait states before that reader, where eight are
+// due; along the other they had passed. A branch that passes over no MFMAs got its wait states on both ways. So no branch stands
+// inside a run here, and its results are held back in one place before any that follows.
 template <int N>
 __device__ __forceinline__ void pa_settle(pa_f4 (&x)[N]) {
   static_assert(N == 2 || N == 4 || N == 8);
@@ -811,7 +816,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   if (d == 0) to.write_lse(p, m, l);
 }
 
-// How a call is cut. waves: of a workgroup, each with 16 rows of the row group; they share one read of the keys (32 tokens of 16
+// How a call is cut: by the table's width, since the lengths are known on the GPU only. (Its figures are of tables as long as the
+// sequences; short ones in a wide table go the way of long ones: 100 keys of 16 heads 6.7 us, 10.3 in a table for 8192, 4 times 300
+// keys of 20 heads 8.0 and 11.3.) waves: of a workgroup, each with 16 rows of the row group; they share one read of the keys (32 tokens of 16
 // heads, 8 sequences of 8000 keys of 64 values: 58 us, 97 with a wave a workgroup; 4 tokens of 8 heads a kv head, 16 sequences of
 // 25 000 keys of 128: 173 and 265; 48 rows on three waves 64 us, on four 77). split: waves that share an item's blocks.
 // workgroups: 0, one an item, or the parts of a balanced line.

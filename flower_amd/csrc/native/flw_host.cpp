@@ -432,7 +432,8 @@ int32_t* i32(const OptTensor& t) { return t ? i32(*t) : nullptr; }
 float* f32(const OptTensor& t) { return t ? f32(*t) : nullptr; }
 int cache_code(const Tensor& pages) { return pages.scalar_type() == at::kBFloat16 ? FLW_BF16 : FLW_E4M3; }
 
-// in_place, where a dimension of one has whatever stride.
+// (B, heads, T, D) as the kernels read it, and its strides: x itself where its rows are contiguous and 16-byte aligned (a
+// dimension of one may have whatever stride), else a copy.
 Tensor heads(const Tensor& x, int64_t* st) {
   const int64_t vec = x.scalar_type() == at::kFloat ? 4 : 8;
   bool ok = x.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;

@@ -56,7 +56,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     i = lens[b] - counts[b] + t and sees the keys j <= i, with i - j < window when a window is given (window <= 0: none, the
     result is zero). H is a multiple of the pool's kv heads: query head h reads kv head h // (H / KV). scale: of the scores,
     1 / sqrt(D) by default. A query without keys, and a padding token, gives zeros (lse -inf). Softmax and sums in fp32; an
-    e4m3 cache's codes are multiplied as they are. Made for few tokens a sequence: up to 64 rows (T H / KV) of a kv head read
+    e4m3 cache's codes are multiplied as they are. Keys and values that are not finite reach only the rows that see them (where an
+    infinite value may come out as NaN). The work is cut by the width of ``tables``, which must be contiguous: narrower
+    ones serve short sequences faster. Made for few tokens a sequence: up to 64 rows (T H / KV) of a kv head read
     the cache once, each further 64 read it again. Forward-only.
     """
     out, lse = _lib.native().paged_attention(q, k_pages, v_pages, tables, lens, counts, _FULL if window is None else window,
