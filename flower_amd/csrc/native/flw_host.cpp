@@ -421,9 +421,11 @@ void check_ints(const char* name, const Tensor& t, at::IntArrayRef sizes, const 
 }
 
 // A derivative of t is asked for in reverse mode (backward); in forward mode, which no operator here has: none is dropped.
-bool wants_backward(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// (A tensor that autograd never touched, most of them, has no record to ask.)
+bool plain(const Tensor& t) { return t.unsafeGetTensorImpl()->autograd_meta() == nullptr; }
+bool wants_backward(const Tensor& t) { return !plain(t) && t.requires_grad() && c10::GradMode::is_enabled(); }
 void refuse_tangent(const char* what, const Tensor& t) {
-  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+  if (!plain(t) && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
     throw std::runtime_error(text(what, " has no forward-mode derivative: call it on tensors without a tangent"));
 }
 
