@@ -282,7 +282,7 @@ class RotaryEmbedding(nn.Module):
     def _kept(self, kind: str, seq_len: int, dtype, device, make):
         """The first seq_len rows of the tables of ``kind``, made by make(rows) where there are none so long. What was handed out
         stays where it is as long as the module lives: a captured graph reads it there on every replay. Longer tables come
-        besides, at least twice as long as the last ones, so that few do. Never inference tensors: training saves them."""
+        besides, twice as long as the last ones or as long as the module's own, so that few do. Never inference tensors: training saves them."""
         key = kind, dtype, torch.device(device)
         last = self._last.get(key)
         if last is not None and last[0] == seq_len and last[1] is self.cos:

@@ -25,7 +25,7 @@ struct PagesParams {
   int32_t* lens_out;
   int32_t* refs_out;
   int32_t* granted;               // reserve
-  int32_t* kept;                  // reorder, or NULL: 1 where place s holds what stood at its parent, 0 where it is empty instead
+  int32_t* kept;                  // reorder, or NULL: 1 where place s holds positions of its parent, 0 where it is empty
   int32_t* need;                  // workspace: [S] pages wanted, -1 where the request cannot be met at all
   int32_t* pairs;                 // workspace: [S][3] dst, src, tokens to copy (dst -1: nothing)
   int32_t* list;                  // workspace: [P] free pages in ascending order
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(256) void reorder_rows_kernel(PagesParams p) {
     p.pairs[3 * s + 1] = copies ? src : -1;
     p.pairs[3 * s + 2] = used;
     p.lens_out[s] = len;
-    if (p.kept != nullptr) p.kept[s] = real;
+    if (p.kept != nullptr) p.kept[s] = len > 0;
   }
 }
 

@@ -11,8 +11,9 @@
 //
 // Measured: rotary of 2 x 8192 tokens, 20 + 20 heads of 64 (168 MB): 31 us, 5.4 TB/s; with q and k read through the caches 36. In
 // fp32 (336 MB), which reads through the caches, 77 us, 4.4 TB/s.
-// Appending 8192 tokens of 16 + 4 + 4 heads of 128 to an e4m3 cache (92 MB): 25 us, 3.6 TB/s (to a bf16 one 19 us, 5.3); with q's, k's and v's heads in one
-// loop 27, read past the caches 30 and more (half layout: a line is read in two parts). A decode step's append: 5 us, its launch.
+// Appending 8192 tokens of 16 + 4 + 4 heads of 128 to an e4m3 cache (92 MB): 25 us, 3.6 TB/s (to a bf16 one 19 us, 5.3);
+// with q's, k's and v's heads in one loop 27, read past the caches 30 and more (half layout: a line is read in two parts). A decode
+// step's append: 5 us, its launch.
 
 #include "flw_common.h"
 

@@ -88,8 +88,8 @@ def reorder_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Te
     first), each other child gets a free page (the lowest numbers first, in the order of s) and a copy of its positions, in
     the pools of all layers: k_pages (layers, pages, ..), v_pages, or one layer's. A place whose page cannot be had is
     emptied: its lens is 0. Pages that nobody holds any more can be taken in the same call. out: as in ``reserve_pages``.
-    ``return_kept`` adds kept (S,) int32: 1 where place s holds its copy (an empty sequence's, too), 0 where it was to be
-    emptied or is for want of a page.
+    ``return_kept`` adds kept (S,) int32: 1 where place s holds positions of its parent, 0 where it is empty: for want of a page,
+    because it was to be emptied, or as its parent was.
     """
     *state, kept = _lib.native().reorder_pages(k_pages, v_pages, tables, lens, refs, parents, out, return_kept,
                                                _lib.stream_or_none(tables))

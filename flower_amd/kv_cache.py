@@ -117,9 +117,9 @@ class PagedKVCache:
 
     def reorder(self, parents) -> torch.Tensor:
         """Place s becomes a copy of the sequence at parents[s], or empty (-1), as ``reorder_pages`` does; returns its kept (S,)
-        int32, on the GPU: 0 for a place that was to be emptied, and for one whose copy found no page and that is empty, too.
-        Such a place must not go on as its parent: ``reserve(kept)`` gives one more token to the others only. ``counts`` is then
-        of no sequence: ``reserve`` comes next."""
+        int32, on the GPU: 0 for an empty place, as one is whose copy found no page. Such a place must not go on as its parent:
+        ``reserve(kept)`` gives one more token to the others only, on this step and on the next ones. ``counts`` is then of no
+        sequence: ``reserve`` comes next."""
         *_, kept = reorder_pages(self.k_pages, self.v_pages, self.tables, self.lens, self.refs, self._ints(parents),
                                  out=(self.tables, self.lens, self.refs), return_kept=True)
         self.counts.zero_()

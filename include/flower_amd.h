@@ -519,8 +519,8 @@ int flw_reserve_pages(const int32_t* tables, const int32_t* lens, const int32_t*
  * free, and a beam search's reordering. Full pages are shared; a last page that is not full stays with one child (the one in
  * its parent's place, else the first), the others get a page of their own with its positions copied, in all L layers of the
  * pools (L, num_pages, ...). A place whose page cannot be had is emptied (lens 0). The outputs may be the inputs.
- * flw_reorder_pages_kept: kept (S, may be NULL) int32 besides, 1 where place s holds its copy (an empty sequence's, too), 0 where
- * it was to be emptied or is for want of a page. */
+ * flw_reorder_pages_kept: kept (S, may be NULL) int32 besides, 1 where place s holds positions of its parent, 0 where it is empty:
+ * for want of a page, because it was to be emptied, or as its parent was. */
 size_t flw_reorder_pages_workspace_bytes(int64_t S, int64_t table_cols, int64_t num_pages);
 int flw_reorder_pages(void* k_pages, void* v_pages, int cache_dtype, int64_t L, int64_t num_pages, int64_t KV,
                       int64_t page_size, int64_t D, const int32_t* tables, const int32_t* lens, const int32_t* refs,
