@@ -15,7 +15,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libflower_amd.so")
 
-F32, BF16, E4M3 = 0, 1, 2
+F32, BF16, E4M3, I8 = 0, 1, 2, 3
 SCALE_TENSOR, SCALE_HEAD, SCALE_BH, SCALE_COLUMN = 0, 1, 2, 3
 LAYOUT_BHTD, LAYOUT_VTILE, LAYOUT_BTHD = 0, 1, 2
 GEMM_A8W8, GEMM_W8A16 = 0, 1
@@ -166,6 +166,17 @@ SIGNATURES = {
                                      c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "flw_fp8_scaled_mm": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                   c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "flw_rows8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "flw_rows8_rmsnorm": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int, c_float,
+                                  c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "flw_rows8_gelu": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "flw_rows8_swiglu": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64,
+                                 c_void_p, c_void_p]),
+    "flw_int8_scaled_mm": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                   c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "flw_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "flw_int8_linear": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "flw_fp8_scaled_mm_residual": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                            c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
 }

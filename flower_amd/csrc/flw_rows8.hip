@@ -1,0 +1,305 @@
+// Rows of activations or weights in 8 bits with one fp32 scale a row, straight from what produces them:
+//   h = x | rmsnorm(x) w | rmsnorm(x + a) w | gelu(x) | silu(x) b
+//   s = max(max|h| / Q, 1e-12), Q = 127 (int8) or 448 (e4m3);  code = rne(h / s), the quotient in fp32.
+// The sum x + a is the residual stream: it is rounded to x's type, written, and the norm is of the rounded sum, which is what
+// the next layer and a backward pass read. h itself stays in fp32 up to its code: rounded to bf16 first, as the separate norm
+// and cast would, values near the row's maximum were off by half an int8 step more. e4m3 codes of h can therefore differ in
+// the last place from flw_rmsnorm_quant_rows_e4m3's, which keeps that rounding.
+// int8 holds no NaN: a row whose maximum is not finite gets the scale NaN and codes 0, so its products are NaN. e4m3 rows
+// do as flw_quant_rows_e4m3's.
+//
+// One pass over memory. A row is held by LPR lanes (64, 256 or 1024 threads), each up to four chunks of 8 values in
+// registers, between the loads, the sum of squares, the maximum and the codes; wider rows are refused. Bound by HBM for many rows, by the latency of
+// load, reduction, reduction, store for few.
+#include "flw_common.h"
+
+namespace flw {
+
+constexpr int kRows8None = 0, kRows8Norm = 1, kRows8AddNorm = 2, kRows8Gelu = 3, kRows8Swiglu = 4;
+constexpr int64_t kRows8MaxCols = 32768;
+
+struct Rows8Params {
+  const void* x;
+  const void* b;           // the residual's addend (AddNorm), or up (Swiglu)
+  const void* w;           // norm weight
+  void* sum;               // x + b (AddNorm)
+  uint8_t* codes;          // [rows, cols], row stride cs
+  float* scale;
+  int64_t rows, xs, bs, ss, cs;
+  int cols;
+  float eps;
+  int w32;                 // the weight is fp32 beside bf16 rows
+  int e4m3;
+};
+
+// 8 values from column c (c < cols) of a row, zeros past the row's end. ALIGNED: cols % 8 == 0 and 16-byte rows; else the
+// loads are by element-aligned vectors (which gfx950 takes at any address), the row's last values one by one.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void rows8_load(const T* row, int c, int cols, float* f) {
+  struct __attribute__((packed, aligned(sizeof(T)))) V { uint32_t w[4]; };
+  constexpr int N = Vec16<T>::N;
+  if (ALIGNED || c + 8 <= cols) {
+#pragma unroll
+    for (int j = 0; j < 8; j += N) {
+      uint4 q;
+      if constexpr (ALIGNED) {
+        q = *reinterpret_cast<const uint4*>(row + c + j);
+      } else {
+        const V v = *reinterpret_cast<const V*>(row + c + j);
+        q = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+      }
+      Vec16<T>::unpack(q, f + j);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v = 0.0f;
+      if (c + j < cols) {
+        if constexpr (sizeof(T) == 2) v = bf16_to_f32(row[c + j]);
+        else v = row[c + j];
+      }
+      f[j] = v;
+    }
+  }
+}
+
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void rows8_store(T* row, int c, int cols, const float* f) {
+  if constexpr (ALIGNED && sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(row + c) = make_uint4(bf16x2_rne(f[0], f[1]), bf16x2_rne(f[2], f[3]), bf16x2_rne(f[4], f[5]),
+                                                    bf16x2_rne(f[6], f[7]));
+  } else if constexpr (ALIGNED) {
+    *reinterpret_cast<float4*>(row + c) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(row + c + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) {
+        if constexpr (sizeof(T) == 2) row[c + j] = (uint16_t)f32_to_bf16_bits(f[j]);
+        else row[c + j] = f[j];
+      }
+  }
+}
+
+// One value of every lane of a row, combined over the row's LPR lanes (the same bits in all of them).
+template <int LPR, typename F>
+__device__ __forceinline__ uint32_t rows8_reduce(uint32_t v, uint32_t* red, F f) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = f(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  if constexpr (LPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < LPR / 64; ++i) v = f(v, red[i]);
+  }
+  return v;
+}
+
+template <typename T, int OP, int LPR, int NC, bool ALIGNED>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Params p) {
+  __shared__ uint32_t red[2][LPR > 64 ? LPR / 64 : 1];
+  constexpr int RPB = LPR > 64 ? 1 : 4;            // rows a workgroup
+  const int64_t row = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / LPR : 0);
+  if (row >= p.rows) return;                       // uniform over a row's lanes
+  const int lane = threadIdx.x % LPR, cols = p.cols;
+  const T* x = static_cast<const T*>(p.x) + row * p.xs;
+  float f[NC][8];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = 8 * (lane + LPR * i);
+    if (c < cols) {
+      rows8_load<T, ALIGNED>(x, c, cols, f[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.0f;
+    }
+  }
+  if constexpr (OP == kRows8AddNorm || OP == kRows8Swiglu) {
+    const T* b = static_cast<const T*>(p.b) + row * p.bs;
+    float g[NC][8];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = 8 * (lane + LPR * i);
+      if (c < cols) rows8_load<T, ALIGNED>(b, c, cols, g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = 8 * (lane + LPR * i);
+      if (c >= cols) continue;
+      if constexpr (OP == kRows8AddNorm) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] = round_to<T>(f[i][e] + g[i][e]);
+        rows8_store<T, ALIGNED>(static_cast<T*>(p.sum) + row * p.ss, c, cols, f[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] / (1.0f + expf(-f[i][e])) * g[i][e];
+      }
+    }
+  }
+  if constexpr (OP == kRows8Norm || OP == kRows8AddNorm) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(f[i][e], f[i][e], ss);
+    ss = __uint_as_float(rows8_reduce<LPR>(__float_as_uint(ss), red[0], [](uint32_t a, uint32_t b) {
+      return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+    const float r = 1.0f / __builtin_sqrtf(ss / (float)cols + p.eps);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = 8 * (lane + LPR * i);
+      if (c >= cols) continue;
+      float g[8];
+      if (sizeof(T) == 2 && p.w32) rows8_load<float, ALIGNED>(static_cast<const float*>(p.w), c, cols, g);
+      else rows8_load<T, ALIGNED>(static_cast<const T*>(p.w), c, cols, g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * r * g[e];
+    }
+  }
+  if constexpr (OP == kRows8Gelu) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.5f * f[i][e] * (1.0f + erff(f[i][e] * 0.70710678118654752f));
+  }
+  uint32_t m = 0;                                  // |h| as bit patterns: NaN above infinity above the rest
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { const uint32_t a = abs_bits(f[i][e]); m = m > a ? m : a; }
+  m = rows8_reduce<LPR>(m, red[1], [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+  const float amax = __uint_as_float(m);
+  const bool finite = m < 0x7F800000u;
+  float s = amax / (p.e4m3 ? kE4m3Max : 127.0f);
+  s = s < kEps ? kEps : s;                         // NaN stays
+  if (!p.e4m3 && !finite) s = __uint_as_float(0x7FC00000u);
+  if (lane == 0) p.scale[row] = s;
+  const float rcp = 1.0f / s;
+  uint8_t* dst = p.codes + row * p.cs;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = 8 * (lane + LPR * i);
+    if (c >= cols) continue;
+    uint32_t w[2] = {0, 0};
+    if (!p.e4m3) {
+      if (finite) {
+        // rne(q) lies in the low byte of q + 1.5 2^23, in two's complement
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w[e >> 2] |= (__float_as_uint(div_by_scale(f[i][e], s, rcp) + 12582912.0f) & 0xFFu) << (8 * (e & 3));
+      }
+    } else if (finite) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        int t = __builtin_amdgcn_cvt_pk_fp8_f32(div_by_scale(f[i][e], s, rcp), div_by_scale(f[i][e + 1], s, rcp), 0, false);
+        w[e >> 2] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(div_by_scale(f[i][e + 2], s, rcp), div_by_scale(f[i][e + 3], s, rcp),
+                                                             t, true);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e >> 2] |= (f32_to_e4m3(f[i][e] / s) & 0xFFu) << (8 * (e & 3));
+    }
+    if constexpr (ALIGNED) {
+      *reinterpret_cast<uint2*>(dst + c) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < cols) dst[c + e] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+    }
+  }
+}
+
+template <typename T, int OP, bool ALIGNED>
+static const void* rows8_of(int lpr, int nc) {
+#define FLW_ROWS8(L, N) reinterpret_cast<const void*>(&rows8_kernel<T, OP, L, N, ALIGNED>)
+  static const void* const table[3][4] = {{FLW_ROWS8(64, 1), FLW_ROWS8(64, 2), FLW_ROWS8(64, 3), FLW_ROWS8(64, 4)},
+                                          {FLW_ROWS8(256, 1), FLW_ROWS8(256, 2), FLW_ROWS8(256, 3), FLW_ROWS8(256, 4)},
+                                          {FLW_ROWS8(1024, 1), FLW_ROWS8(1024, 2), FLW_ROWS8(1024, 3), FLW_ROWS8(1024, 4)}};
+#undef FLW_ROWS8
+  return table[lpr == 64 ? 0 : lpr == 256 ? 1 : 2][nc - 1];
+}
+
+static bool rows_ok(const void* p, int64_t stride, int64_t cols, size_t size) {
+  return p != nullptr && stride >= cols && (uintptr_t)p % size == 0;
+}
+static bool rows16(const void* p, int64_t stride, size_t size) {
+  return p == nullptr || ((uintptr_t)p % 16 == 0 && stride * (int64_t)size % 16 == 0);
+}
+
+template <int OP>
+static int rows8(Rows8Params p, int dtype, int64_t cols, int weight_dtype, int code_type, void* stream, const char* name) {
+  FLW_REQUIRE(dtype == FLW_F32 || dtype == FLW_BF16, FLW_E_UNSUPPORTED, "dtype %d not supported (f32=0, bf16=1)", dtype);
+  FLW_REQUIRE(code_type == FLW_I8 || code_type == FLW_E4M3, FLW_E_UNSUPPORTED, "codes must be int8 or e4m3, got %d", code_type);
+  FLW_REQUIRE(p.rows >= 0 && cols > 0, FLW_E_INVALID, "empty or negative shape (%lld, %lld)", (long long)p.rows, (long long)cols);
+  FLW_REQUIRE(cols <= kRows8MaxCols, FLW_E_UNSUPPORTED, "rows of at most %lld values, got %lld", (long long)kRows8MaxCols,
+              (long long)cols);
+  FLW_REQUIRE(p.rows <= 0x7FFFFFFFll, FLW_E_UNSUPPORTED, "too many rows");
+  const size_t size = dtype == FLW_F32 ? 4 : 2;
+  if (p.rows == 0) return FLW_OK;
+  FLW_REQUIRE(rows_ok(p.x, p.xs, cols, size) && rows_ok(p.codes, p.cs, cols, 1) && rows_ok(p.scale, cols, cols, 4), FLW_E_INVALID,
+              "null or misaligned pointer, or a row stride below the row");
+  if (OP == kRows8AddNorm || OP == kRows8Swiglu)
+    FLW_REQUIRE(rows_ok(p.b, p.bs, cols, size), FLW_E_INVALID, "the second input: null, misaligned, or a row stride below the row");
+  if (OP == kRows8AddNorm)
+    FLW_REQUIRE(rows_ok(p.sum, p.ss, cols, size), FLW_E_INVALID, "the sum: null, misaligned, or a row stride below the row");
+  if (OP == kRows8Norm || OP == kRows8AddNorm) {
+    FLW_REQUIRE(weight_dtype == dtype || weight_dtype == FLW_F32, FLW_E_UNSUPPORTED, "the weight must be fp32 or of the rows' type");
+    p.w32 = weight_dtype == FLW_F32;
+    FLW_REQUIRE(rows_ok(p.w, cols, cols, p.w32 ? 4 : 2), FLW_E_INVALID, "the weight is null or misaligned");
+    FLW_REQUIRE(p.eps >= 0.0f, FLW_E_INVALID, "eps must be non-negative");
+  }
+  p.cols = (int)cols;
+  p.e4m3 = code_type == FLW_E4M3;
+  const bool aligned = cols % 8 == 0 && rows16(p.x, p.xs, size) && rows16(p.b, p.bs, size) && rows16(p.sum, p.ss, size) &&
+                       rows16(p.w, 0, 4) && (uintptr_t)p.codes % 8 == 0 && p.cs % 8 == 0;
+  // The fewest lanes whose four chunks hold the row.
+  const int lpr = cols <= 2048 ? 64 : cols <= 8192 ? 256 : 1024;
+  const int nc = (int)((cols + 8 * lpr - 1) / (8 * lpr));
+  const void* kernel = dtype == FLW_F32 ? (aligned ? rows8_of<float, OP, true>(lpr, nc) : rows8_of<float, OP, false>(lpr, nc))
+                                        : (aligned ? rows8_of<uint16_t, OP, true>(lpr, nc) : rows8_of<uint16_t, OP, false>(lpr, nc));
+  const int64_t rpb = lpr == 64 ? 4 : 1;
+  (void)launch_timed(kernel, dim3((unsigned)((p.rows + rpb - 1) / rpb)), dim3((unsigned)(lpr == 64 ? 256 : lpr)),
+                     static_cast<hipStream_t>(stream), p);
+  return check_launch(name);
+}
+
+}  // namespace flw
+
+using namespace flw;
+
+extern "C" int flw_rows8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_row_stride, int code_type, void* codes,
+                         int64_t codes_row_stride, float* scale, void* stream) {
+  Rows8Params p{};
+  p.x = x; p.rows = rows; p.xs = x_row_stride; p.codes = static_cast<uint8_t*>(codes); p.cs = codes_row_stride; p.scale = scale;
+  return rows8<kRows8None>(p, dtype, cols, dtype, code_type, stream, "flw_rows8");
+}
+
+extern "C" int flw_rows8_rmsnorm(const void* x, const void* residual, int dtype, int64_t rows, int64_t cols, int64_t x_row_stride,
+                                 int64_t residual_row_stride, const void* weight, int weight_dtype, float eps, void* sum,
+                                 int64_t sum_row_stride, int code_type, void* codes, int64_t codes_row_stride, float* scale,
+                                 void* stream) {
+  Rows8Params p{};
+  p.x = x; p.rows = rows; p.xs = x_row_stride; p.codes = static_cast<uint8_t*>(codes); p.cs = codes_row_stride; p.scale = scale;
+  p.w = weight; p.eps = eps;
+  if (residual == nullptr) return rows8<kRows8Norm>(p, dtype, cols, weight_dtype, code_type, stream, "flw_rows8_rmsnorm");
+  p.b = residual; p.bs = residual_row_stride; p.sum = sum; p.ss = sum_row_stride;
+  return rows8<kRows8AddNorm>(p, dtype, cols, weight_dtype, code_type, stream, "flw_rows8_rmsnorm");
+}
+
+extern "C" int flw_rows8_gelu(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_row_stride, int code_type,
+                              void* codes, int64_t codes_row_stride, float* scale, void* stream) {
+  Rows8Params p{};
+  p.x = x; p.rows = rows; p.xs = x_row_stride; p.codes = static_cast<uint8_t*>(codes); p.cs = codes_row_stride; p.scale = scale;
+  return rows8<kRows8Gelu>(p, dtype, cols, dtype, code_type, stream, "flw_rows8_gelu");
+}
+
+extern "C" int flw_rows8_swiglu(const void* gate, const void* up, int dtype, int64_t rows, int64_t cols, int64_t gate_row_stride,
+                                int64_t up_row_stride, int code_type, void* codes, int64_t codes_row_stride, float* scale,
+                                void* stream) {
+  Rows8Params p{};
+  p.x = gate; p.rows = rows; p.xs = gate_row_stride; p.codes = static_cast<uint8_t*>(codes); p.cs = codes_row_stride; p.scale = scale;
+  p.b = up; p.bs = up_row_stride;
+  return rows8<kRows8Swiglu>(p, dtype, cols, dtype, code_type, stream, "flw_rows8_swiglu");
+}

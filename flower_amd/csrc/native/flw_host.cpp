@@ -5,7 +5,7 @@
 // its autograd node and its module stay in Python, and every function takes the stream it launches on
 // (torch's current stream of the tensors' device, as a handle). The rotary positions and the paged
 // cache's operators are here as a whole, their checks and the one's autograd node too: their kernels
-// take 3 to 6 us in a decode step, less than the same checks take in Python.
+// take 3 to 6 us in a decode step, less than the same checks take in Python; and so are the 8-bit rows and the int8 product.
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
@@ -750,6 +750,190 @@ std::tuple<Tensor, Tensor, Tensor> compact_pages(const Tensor& k_pages, const Te
   return {to[0], to[1], live};
 }
 
+// ---------------------------------------------------------------- 8-bit rows, int8 linear
+// Checked here too, on the device of their tensors.
+
+// x (.., K) as rows [R, K] with one row stride: x itself where its layout has one, else a copy.
+Tensor as_rows(const Tensor& x, int64_t* ld) {
+  const int64_t K = x.size(-1);
+  Tensor y = x.dim() == 2 ? x : x.reshape({-1, K});
+  auto bad = [K](const Tensor& t) { return (K > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < K); };
+  if (bad(y)) y = y.clone(at::MemoryFormat::Contiguous);
+  *ld = y.size(0) > 1 ? y.stride(0) : K;
+  return y;
+}
+
+at::ScalarType code_dtype(bool e4m3) { return e4m3 ? at::kFloat8_e4m3fn : at::kChar; }
+
+void check_float_rows(const char* what, const Tensor& x) {
+  REFUSE_UNLESS(x.dim() >= 1 && x.size(-1) > 0, what, " takes rows (.., K), K > 0, got ", x.sizes());
+  if (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat)
+    throw py::type_error(text(what, " takes bfloat16 or float32 rows; got ", x.scalar_type()));
+  refuse_gradients(what, x);
+}
+void check_like(const char* what, const char* name, const Tensor& t, const Tensor& x) {
+  REFUSE_UNLESS(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device(), what, ": ", name,
+                " must be ", x.sizes(), " ", x.scalar_type(), " on ", x.device(), " as the rows, got ", t.sizes(), " ", t.scalar_type(),
+                " on ", t.device());
+  refuse_gradients(what, t);
+}
+
+// The codes (.., K) and scales (..) that a pass over the rows x writes: launch(rows, codes, scale).
+struct Rows8 {
+  Tensor codes, scale;
+  Rows8(const Tensor& x, bool e4m3)
+      : codes(empty(x, x.sizes(), code_dtype(e4m3))), scale(empty(x, x.sizes().slice(0, x.dim() - 1), at::kFloat)) {}
+};
+
+std::tuple<Tensor, Tensor> quant_rows8(const Tensor& x, bool e4m3, int64_t stream) {
+  check_float_rows("quant_rows", x);
+  require_gpu(x);
+  c10::DeviceGuard guard(x.device());
+  int64_t xs;
+  const Tensor r = as_rows(x, &xs);
+  Rows8 out(x, e4m3);
+  const int64_t K = x.size(-1);
+  check(flw_rows8(r.data_ptr(), dtype_code(r), r.size(0), K, xs, e4m3 ? FLW_E4M3 : FLW_I8, out.codes.data_ptr(), K, f32(out.scale),
+                  str(stream)),
+        "quant_rows");
+  return {out.codes, out.scale};
+}
+
+std::tuple<Tensor, Tensor, OptTensor> rms_norm_quant(const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual,
+                                                     bool e4m3, int64_t stream) {
+  check_float_rows("rms_norm_quant", x);
+  const int64_t K = x.size(-1);
+  REFUSE_UNLESS(weight.dim() == 1 && weight.size(0) == K && weight.device() == x.device() &&
+                    (weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat),
+                "rms_norm_quant: the weight must be (", K, ",), of the rows' type or float32, on ", x.device(), ", got ", weight.sizes(),
+                " ", weight.scalar_type(), " on ", weight.device());
+  REFUSE_UNLESS(eps >= 0.0, "eps must be non-negative");
+  refuse_gradients("rms_norm_quant", weight);
+  if (residual) check_like("rms_norm_quant", "residual", *residual, x);
+  require_gpu(x);
+  c10::DeviceGuard guard(x.device());
+  int64_t xs, as = 0;
+  const Tensor r = as_rows(x, &xs), w = weight.contiguous();
+  Tensor a;
+  OptTensor sum;
+  if (residual) {
+    a = as_rows(*residual, &as);
+    sum = empty(x, x.sizes(), x.scalar_type());
+  }
+  Rows8 out(x, e4m3);
+  check(flw_rows8_rmsnorm(r.data_ptr(), residual ? a.data_ptr() : nullptr, dtype_code(r), r.size(0), K, xs, as, w.data_ptr(),
+                          dtype_code(w), (float)eps, opt(sum), K, e4m3 ? FLW_E4M3 : FLW_I8, out.codes.data_ptr(), K, f32(out.scale),
+                          str(stream)),
+        "rms_norm_quant");
+  return {out.codes, out.scale, sum};
+}
+
+// gelu(x), or with up silu(x) up.
+std::tuple<Tensor, Tensor> act_quant(const Tensor& x, const OptTensor& up, bool e4m3, int64_t stream) {
+  const char* what = up ? "swiglu_quant" : "gelu_quant";
+  check_float_rows(what, x);
+  if (up) check_like(what, "up", *up, x);
+  require_gpu(x);
+  c10::DeviceGuard guard(x.device());
+  const int64_t K = x.size(-1);
+  int64_t xs, us = 0;
+  const Tensor r = as_rows(x, &xs);
+  Rows8 out(x, e4m3);
+  const int type = e4m3 ? FLW_E4M3 : FLW_I8;
+  if (up) {
+    const Tensor u = as_rows(*up, &us);
+    check(flw_rows8_swiglu(r.data_ptr(), u.data_ptr(), dtype_code(r), r.size(0), K, xs, us, type, out.codes.data_ptr(), K,
+                           f32(out.scale), str(stream)),
+          what);
+  } else {
+    check(flw_rows8_gelu(r.data_ptr(), dtype_code(r), r.size(0), K, xs, type, out.codes.data_ptr(), K, f32(out.scale), str(stream)),
+          what);
+  }
+  return {out.codes, out.scale};
+}
+
+// What the int8 product and linear share: weights b (N, K) and their scales, bias and residual, and the output (.., N).
+struct Int8Args {
+  Tensor b, bias, res, y;
+  int64_t M, N, K, bs, rs = 0;
+  std::vector<int64_t> shape;
+  Int8Args(const char* what, const Tensor& a, const Tensor& b0, const Tensor& b_scale, const OptTensor& bias0, const OptTensor& res0) {
+    K = a.size(-1);
+    REFUSE_UNLESS(b0.dim() == 2 && b0.scalar_type() == at::kChar && b0.size(1) == K && b0.size(0) > 0 && b0.device() == a.device(),
+                  what, ": the weight must be int8 (N, ", K, ") on ", a.device(), ", got ", b0.sizes(), " ", b0.scalar_type(), " on ",
+                  b0.device());
+    N = b0.size(0);
+    M = a.numel() / K;
+    check_scale(what, "weight_scale", b_scale, N, a);
+    shape = a.sizes().vec();
+    shape.back() = N;
+    if (bias0) {
+      REFUSE_UNLESS(bias0->dim() == 1 && bias0->size(0) == N && bias0->device() == a.device() &&
+                        (bias0->scalar_type() == at::kFloat || bias0->scalar_type() == at::kBFloat16),
+                    what, ": the bias must be bfloat16 or float32 (", N, ",) on ", a.device(), ", got ", bias0->sizes(), " ",
+                    bias0->scalar_type(), " on ", bias0->device());
+      refuse_gradients(what, *bias0);
+    }
+    if (res0) {
+      REFUSE_UNLESS(res0->sizes() == at::IntArrayRef(shape) && res0->scalar_type() == at::kBFloat16 && res0->device() == a.device(),
+                    what, ": the residual must be bfloat16 ", at::IntArrayRef(shape), " on ", a.device(), ", got ", res0->sizes(), " ",
+                    res0->scalar_type(), " on ", res0->device());
+      refuse_gradients(what, *res0);
+    }
+    require_gpu(a);
+  }
+  static void check_scale(const char* what, const char* name, const Tensor& t, int64_t rows, const Tensor& with) {
+    REFUSE_UNLESS(t.scalar_type() == at::kFloat && (t.numel() == rows || t.numel() == 1) && t.is_contiguous() &&
+                      t.device() == with.device(),
+                  what, ": ", name, " must be contiguous float32, ", rows, " or one, on ", with.device(), ", got ", t.sizes(), " ",
+                  t.scalar_type(), " on ", t.device());
+    refuse_gradients(what, t);
+  }
+  void lay_out(const Tensor& like, const OptTensor& bias0, const OptTensor& res0, const Tensor& b0) {
+    b = as_rows(b0, &bs);
+    if (bias0) bias = bias0->contiguous();
+    if (res0) res = as_rows(*res0, &rs);
+    y = empty(like, shape, at::kBFloat16);
+  }
+  void* bias_ptr() const { return bias.defined() ? bias.data_ptr() : nullptr; }
+  int bias_code() const { return bias.defined() ? dtype_code(bias) : FLW_BF16; }
+  void* res_ptr() const { return res.defined() ? res.data_ptr() : nullptr; }
+};
+
+Tensor int8_scaled_mm(const Tensor& a0, const Tensor& a_scale, const Tensor& b0, const Tensor& b_scale, const OptTensor& bias,
+                      const OptTensor& residual, int64_t stream) {
+  REFUSE_UNLESS(a0.dim() >= 1 && a0.size(-1) > 0, "int8_scaled_mm takes rows (.., K), K > 0, got ", a0.sizes());
+  if (a0.scalar_type() != at::kChar) throw py::type_error(text("int8_scaled_mm takes int8 codes; got ", a0.scalar_type()));
+  Int8Args::check_scale("int8_scaled_mm", "a_scale", a_scale, a0.numel() / a0.size(-1), a0);
+  Int8Args p("int8_scaled_mm", a0, b0, b_scale, bias, residual);
+  c10::DeviceGuard guard(a0.device());
+  int64_t as;
+  const Tensor a = as_rows(a0, &as);
+  p.lay_out(a0, bias, residual, b0);
+  check(flw_int8_scaled_mm(static_cast<const int8_t*>(a.data_ptr()), p.M, p.K, as, static_cast<const int8_t*>(p.b.data_ptr()), p.N,
+                           p.bs, f32(a_scale), a_scale.numel(), f32(b_scale), b_scale.numel(), p.bias_ptr(), p.bias_code(), p.res_ptr(),
+                           p.rs, p.y.data_ptr(), p.N, str(stream)),
+        "int8_scaled_mm");
+  return p.y;
+}
+
+Tensor int8_linear(const Tensor& x0, const Tensor& b0, const Tensor& b_scale, const OptTensor& bias, const OptTensor& residual,
+                   int64_t stream) {
+  check_float_rows("int8_linear", x0);
+  Int8Args p("int8_linear", x0, b0, b_scale, bias, residual);
+  c10::DeviceGuard guard(x0.device());
+  int64_t xs;
+  const Tensor x = as_rows(x0, &xs);
+  p.lay_out(x0, bias, residual, b0);
+  const size_t need = flw_int8_linear_workspace_bytes(p.M, p.K);
+  const Tensor ws = workspace(x0, need);
+  check(flw_int8_linear(x.data_ptr(), dtype_code(x), p.M, p.K, xs, static_cast<const int8_t*>(p.b.data_ptr()), p.N, p.bs, f32(b_scale),
+                        b_scale.numel(), p.bias_ptr(), p.bias_code(), p.res_ptr(), p.rs, p.y.data_ptr(), p.N, ws.data_ptr(),
+                        (size_t)ws.numel(), str(stream)),
+        "int8_linear");
+  return p.y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -791,4 +975,9 @@ PYBIND11_MODULE(_native, m) {
   m.def("reserve_pages", &reserve_pages, nogil());
   m.def("reorder_pages", &reorder_pages, nogil());
   m.def("compact_pages", &compact_pages, nogil());
+  m.def("quant_rows8", &quant_rows8, nogil());
+  m.def("rms_norm_quant", &rms_norm_quant, nogil());
+  m.def("act_quant", &act_quant, nogil());
+  m.def("int8_scaled_mm", &int8_scaled_mm, nogil());
+  m.def("int8_linear", &int8_linear, nogil());
 }

@@ -1,0 +1,134 @@
+"""Linears in 8-bit integers: int8 weights with a scale a channel, int8 activations with a scale a token.
+
+``Int8Linear``            an ``nn.Linear`` whose forward is ``flower_amd.kernels.int8_linear``. Trainable, straight through
+                          the quantisers: the gradient products are the e4m3 ones of the "rowwise" recipe
+                          (``flower_amd.precision``), whose range a gradient's rows need; ``backward_fp8 = False`` takes bf16.
+``int8_linear_train``     its forward as a function, differentiable in input, weight, bias and residual
+``convert_model_to_int8`` replaces a model's linears as ``convert_model_to_fp8`` does (flower/precision.py:134-195), by the
+                          same rules; ``fp8_weight_cache`` then keeps the int8 codes for the length of its block.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from .kernels.int8 import int8_scaled_mm, quant_rows
+from .precision import Fp8Linear, fp8_linear_backward, fp8_module_filter, quantize_weight_cols
+
+
+def quantize_weight_int8(weight: torch.Tensor):
+    """(codes (N, K) int8, scale (N,) float32) of a weight: one scale an output channel."""
+    return quant_rows(weight.detach())
+
+
+class _Int8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, w8, w_scale, mod):
+        ctx.save_for_backward(x, weight)
+        ctx.mod, ctx.bias_dtype = mod, None if bias is None else bias.dtype
+        return _lib.native().int8_linear(x, w8, w_scale, bias, residual, _lib.stream_or_none(x))
+
+    @staticmethod
+    def backward(ctx, g):
+        x, weight = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        N, K = weight.shape
+        g2, x2 = g.reshape(-1, N), x.reshape(-1, K)
+        gx = gw = gb = None
+        if g2.shape[0] == 0:
+            gx = torch.zeros_like(x) if need_x else None
+            gw = torch.zeros_like(weight) if need_w else None
+        # The e4m3 products take widths in whole 16-byte rows; others, and a module that asks for it, run in bf16.
+        elif (ctx.mod is None or ctx.mod.backward_fp8) and N % 16 == 0 and K % 16 == 0:
+            cols = ctx.mod.weight_col_codes if ctx.mod is not None else lambda: quantize_weight_cols(weight, "rowwise")
+            gx, gw = fp8_linear_backward(g2, x2, cols, "rowwise", need_x, need_w)
+        else:
+            gx = g2 @ weight.to(g2.dtype) if need_x else None
+            gw = g2.t() @ x2.to(g2.dtype) if need_w else None
+        gx = gx.reshape(x.shape).to(x.dtype) if gx is not None else None
+        gw = gw.to(weight.dtype) if gw is not None else None
+        if need_b:
+            gb = g2.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
+        return gx, gw, gb, (g if need_r else None), None, None, None
+
+
+def int8_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                      residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ weight^T + bias``, plus ``residual``, in int8: both operands quantised now, a scale a token and a channel; bf16 out.
+    x (.., K), weight (N, K) bf16 or fp32. Differentiable, as ``Int8Linear`` is."""
+    w8, w_scale = quantize_weight_int8(weight)
+    return _Int8LinearFn.apply(x, weight, bias, residual, w8, w_scale, None)
+
+
+class Int8Linear(Fp8Linear):
+    """``nn.Linear`` in int8 (see the module). Shares the Parameters of the Linear it was built from. The weight is quantised
+    on every call unless an ``fp8_weight_cache`` is active. ``forward_codes`` takes the input as codes and scales already, from
+    ``rms_norm_quant`` or another of the passes of ``flower_amd.kernels``."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None) -> None:
+        super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        self.recipe = "int8"
+
+    @classmethod
+    def from_linear(cls, lin: nn.Linear) -> "Int8Linear":
+        new = super().from_linear(lin)
+        new.recipe = "int8"
+        return new
+
+    def quantize_weight(self):
+        return quantize_weight_int8(self.weight)
+
+    def tensorwise_codes(self):
+        raise RuntimeError("an Int8Linear has no tensorwise codes")
+
+    def weight_col_codes(self):
+        cached = getattr(self, "_fp8_cached_cols", None)
+        if cached is not None:
+            return cached
+        codes = quantize_weight_cols(self.weight, "rowwise")
+        if getattr(self, "_fp8_cached", None) is not None:       # a cache context is active
+            self._fp8_cached_cols = codes
+        return codes
+
+    def forward_with(self, x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, x_amax=None, residual=None,
+                     w8t=None) -> torch.Tensor:
+        """x_amax and w8t are of the tensorwise recipe: not used."""
+        if torch.is_autocast_enabled():
+            x = x.to(torch.get_autocast_gpu_dtype())
+        elif x.dtype not in (torch.bfloat16, torch.float32):
+            x = x.to(torch.bfloat16)
+        return _Int8LinearFn.apply(x, self.weight, self.bias, residual, w8, w_scale, self)
+
+    def forward(self, x: torch.Tensor, x_amax=None, residual=None) -> torch.Tensor:
+        return self.forward_with(x, *self.weight_codes(), residual=residual)
+
+    @torch.no_grad()
+    def forward_codes(self, codes: torch.Tensor, scale: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """The output for an input in int8: codes (.., in_features) and scale (..). Forward-only."""
+        return int8_scaled_mm(codes, scale, *self.weight_codes(), bias=self.bias, residual=residual)
+
+
+def convert_model_to_int8(model: nn.Module, *, keep_bf16_blocks: int = 1, verbose: bool = True):
+    """Replace every Linear that ``fp8_module_filter`` admits by an ``Int8Linear`` sharing its Parameters, in place; returns
+    (model, info). As ``convert_model_to_fp8``, it refuses a model without ``blocks``."""
+    num_layers = len(getattr(model, "blocks", []))
+    if num_layers == 0:
+        raise RuntimeError("convert_model_to_int8 found no `blocks` on the model; the block-range guardrail cannot be applied. "
+                           "Refusing to convert blindly.")
+    admit = fp8_module_filter(num_layers, keep_bf16_blocks)
+    named = list(model.named_modules())
+    targets = [(fqn, m) for fqn, m in named if admit(m, fqn)]
+    for fqn, mod in targets:
+        owner, _, attr = fqn.rpartition(".")
+        setattr(model.get_submodule(owner) if owner else model, attr, Int8Linear.from_linear(mod))
+    info = {"int8_keep_bf16_blocks": keep_bf16_blocks, "int8_converted_linears": len(targets),
+            "int8_total_linears": sum(isinstance(m, nn.Linear) for _, m in named)}
+    if verbose:
+        print(f"[int8] converted {len(targets)}/{info['int8_total_linears']} Linear layers (blocks {keep_bf16_blocks}.."
+              f"{num_layers - keep_bf16_blocks - 1} of {num_layers}; first/last {keep_bf16_blocks} stay as they are)", flush=True)
+    return model, info
+
+
+__all__ = ["Int8Linear", "int8_linear_train", "convert_model_to_int8", "quantize_weight_int8"]

@@ -29,8 +29,9 @@ enum flw_status {
   FLW_E_LAUNCH = 4        /* HIP launch error */
 };
 
-/* FLW_E4M3: what a paged key-value cache may hold besides bf16; the other entry points take e4m3 as codes. */
-enum flw_dtype { FLW_F32 = 0, FLW_BF16 = 1, FLW_E4M3 = 2 };
+/* FLW_E4M3: what a paged key-value cache may hold besides bf16; the other entry points take e4m3 as codes. FLW_I8: codes of
+ * flw_rows8 and its kin. */
+enum flw_dtype { FLW_F32 = 0, FLW_BF16 = 1, FLW_E4M3 = 2, FLW_I8 = 3 };
 
 /* Scale granularity for a (B, H, T, D) tensor: one scale, one per head h (amax over B, T, D),
  * or one per (b, h) slice (amax over T, D). Scale arrays hold 1, H or B*H floats. */
@@ -616,6 +617,51 @@ int flw_fp8_scaled_mm_residual(const uint8_t* x8, int64_t M, int64_t K, const ui
                                const float* x_scale, int64_t x_scale_count, const float* w_scale,
                                int64_t w_scale_count, void* y, int64_t y_row_stride,
                                const void* residual, int64_t residual_row_stride, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit rows and the int8 linear */
+
+/* Rows h [rows, cols] in 8 bits with one fp32 scale a row, from what produces them, in one pass. No counterpart in the
+ * reference, whose 8-bit linears are e4m3 (the cast of flower/models/base.py:912-918 behind RMSNorm, :324-338, GELU, :519-521,
+ * or SwiGLU, :538-550):
+ *   scale = max(max|h| / Q, 1e-12);  code_type FLW_I8: Q = 127, code = rne(h / scale);
+ *                                    FLW_E4M3: Q = 448, code = e4m3_rne(h / scale) (no clamp), quotients in fp32.
+ * h stays in fp32 up to its code. A row that holds a NaN or an infinity: int8 codes 0 and the scale NaN; e4m3 as
+ * flw_quant_rows_e4m3 has it.
+ *   flw_rows8          h = x;
+ *   flw_rows8_rmsnorm  h = t / sqrt(mean(t^2) + eps) * weight[cols], t = x, or with a residual t = x + residual rounded to x's
+ *                      type and written to sum (the sum may not overlap an input);
+ *   flw_rows8_gelu     h = 0.5 x (1 + erf(x / sqrt 2));
+ *   flw_rows8_swiglu   h = gate / (1 + exp(-gate)) * up.
+ * dtype: fp32 or bf16, of x, residual, sum, gate and up; weight fp32 or of that type. Row strides in elements, at least cols,
+ * any alignment (16-byte rows are read faster). cols <= 32768. codes: bytes, row stride at least cols; the bytes behind a row
+ * stay as they are. */
+int flw_rows8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_row_stride, int code_type, void* codes,
+              int64_t codes_row_stride, float* scale, void* stream);
+int flw_rows8_rmsnorm(const void* x, const void* residual, int dtype, int64_t rows, int64_t cols, int64_t x_row_stride,
+                      int64_t residual_row_stride, const void* weight, int weight_dtype, float eps, void* sum,
+                      int64_t sum_row_stride, int code_type, void* codes, int64_t codes_row_stride, float* scale, void* stream);
+int flw_rows8_gelu(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_row_stride, int code_type, void* codes,
+                   int64_t codes_row_stride, float* scale, void* stream);
+int flw_rows8_swiglu(const void* gate, const void* up, int dtype, int64_t rows, int64_t cols, int64_t gate_row_stride,
+                     int64_t up_row_stride, int code_type, void* codes, int64_t codes_row_stride, float* scale, void* stream);
+
+/* y[M, N] (bf16) = (a[M, K] . b[N, K]^T) * a_scale[m] * b_scale[n] + bias[n] of int8 matrices, or bf16(residual + bf16(that)):
+ * the integer form of flw_fp8_scaled_mm (torch._scaled_mm, flower/models/base.py:919-923). The sums are exact in int32
+ * (K <= 131071), the result does not depend on how the work is cut. Scale counts: M or 1, and N or 1. bias: NULL, fp32 or
+ * bf16 (bias_dtype). residual: NULL or bf16. Row strides in elements, any alignment; any sizes (K % 16 == 0 with 16-byte rows
+ * is the fast case). y may not overlap an input. */
+int flw_int8_scaled_mm(const int8_t* a, int64_t M, int64_t K, int64_t a_row_stride, const int8_t* b, int64_t N,
+                       int64_t b_row_stride, const float* a_scale, int64_t a_scale_count, const float* b_scale,
+                       int64_t b_scale_count, const void* bias, int bias_dtype, const void* residual,
+                       int64_t residual_row_stride, void* y, int64_t y_row_stride, void* stream);
+
+/* flw_rows8 (int8) of the rows x [M, K], fp32 or bf16 (dtype), then flw_int8_scaled_mm of them: a linear's forward with int8
+ * weights b [N, K]. workspace: flw_int8_linear_workspace_bytes(M, K), 16-byte aligned (the codes and their scales). */
+size_t flw_int8_linear_workspace_bytes(int64_t M, int64_t K);
+int flw_int8_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t x_row_stride, const int8_t* b, int64_t N,
+                    int64_t b_row_stride, const float* b_scale, int64_t b_scale_count, const void* bias, int bias_dtype,
+                    const void* residual, int64_t residual_row_stride, void* y, int64_t y_row_stride, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

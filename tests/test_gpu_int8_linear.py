@@ -1,0 +1,157 @@
+"""GPU: Int8Linear and int8_linear_train: outputs, gradients, the weight cache.
+
+The gradient is straight through the quantisers, its products the e4m3 ones of the rowwise recipe: against the oracle's, in
+64 bits on the same codes, a result is off by its bf16 rounding, 2^-8, and the matrix unit's fp32 sums (a thousandth of the
+largest is asked, as of the e4m3 linears). Against the gradient of the unquantised linear the two operands' e4m3 rounding, at most
+2^-4 of a value each, uniform within it, is 2^-4 / sqrt 3 * sqrt 2 = 5.1 % of the result's size at the most; 6 % is asked.
+"""
+
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+from flower_amd import int8
+from flower_amd.kernels import int8_linear, quant_rows
+from flower_amd.precision import fp8_weight_cache
+from oracle.gemm import fp8_linear_backward
+from tests.gpu_util import seeded, to_np
+
+pytestmark = pytest.mark.gpu
+
+
+def tensors(M, N, K, dtype=torch.bfloat16):
+    x, w, b = seeded((M, K), 1, dtype), seeded((N, K), 2, dtype, scale=K ** -0.5), seeded((N,), 3, dtype)
+    g = seeded((M, N), 4, torch.bfloat16) * seeded((M, 1), 5, torch.bfloat16).exp()
+    return x, w, b, g
+
+
+def off(a, b):
+    return float(np.linalg.norm(a - b) / np.linalg.norm(b))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 16, 16), (3, 48, 64), (130, 256, 80), (517, 1280, 640)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients(M, N, K, dtype):
+    x, w, b, g = tensors(M, N, K, dtype)
+    r = seeded((M, N), 6, torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    y = int8.int8_linear_train(*leaves)
+    w8, sw = quant_rows(w.detach())
+    assert torch.equal(y.detach(), int8_linear(x.detach(), w8, sw, bias=b.detach(), residual=r.detach()))
+    gx, gw, gb, gr = torch.autograd.grad(y, leaves, g)
+    assert all(t.dtype == s.dtype and t.shape == s.shape for t, s in zip((gx, gw, gb, gr), leaves))
+    half = lambda t: to_np(t.detach().to(torch.bfloat16))  # noqa: E731
+    # the e4m3 casts read the input as it is, the weight too
+    want_x, want_w = fp8_linear_backward(to_np(g), to_np(x), to_np(w), "rowwise")
+    for got, want in ((gx, want_x), (gw, want_w)):
+        assert np.abs(to_np(got) - want).max() <= np.abs(want) .max() * (2.0 ** -8 + 1e-3)
+    assert torch.equal(gr, g)
+    s = g.double().sum(0).cpu().numpy()
+    slack = np.abs(s) * 2.0 ** -8 + g.double().abs().sum(0).cpu().numpy() * M * 2.0 ** -24
+    assert np.all(np.abs(to_np(gb).astype(np.float64) - s) <= slack)
+    assert half(gx).shape == (M, K)
+
+
+def test_gradients_are_near_the_linears_own_and_its_differences():
+    x, w, b, g = tensors(300, 256, 512)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    gx, gw, gb = torch.autograd.grad(int8.int8_linear_train(*leaves), leaves, g)
+    xd, wd, gd = x.detach().double(), w.detach().double(), g.double()
+    for got, want in ((gx, gd @ wd), (gw, gd.t() @ xd)):
+        assert off(got.double().cpu().numpy(), want.cpu().numpy()) < 0.06
+    # along the gradient itself: (f(x + h d) - f(x - h d)) / 2 h of the linear that is quantised
+    for leaf, grad, f in ((xd, gx, lambda t: (t @ wd.t() * gd).sum()), (wd, gw, lambda t: (xd @ t.t() * gd).sum())):
+        d = grad.double() / grad.double().norm()
+        slope = (f(leaf + 1e-3 * d) - f(leaf - 1e-3 * d)) / 2e-3
+        assert abs(slope / (grad.double() * d).sum() - 1) < 0.06
+    # the bias enters the output unquantised: its differences are the output's, to the roundings
+    with torch.no_grad():
+        up, down = (int8.int8_linear_train(x, w, b.float() + s) for s in (4.0, -4.0))
+    slope = ((up.double() - down.double()) * gd).sum() / 8
+    most = (gd.abs() * (up.double().abs() + down.double().abs())).sum() * 2.0 ** -8 / 8
+    assert abs(slope - gb.double().sum()) <= most + gd.abs().sum() * 2.0 ** -8
+
+
+@pytest.mark.parametrize("N,K", [(33, 80), (64, 40), (256, 128)])
+def test_bf16_backward_of_odd_widths_and_on_request(N, K):
+    x, w, b, g = tensors(65, N, K)
+    mod = int8.Int8Linear(K, N, device="cuda", dtype=torch.bfloat16)
+    mod.load_state_dict({"weight": w, "bias": b})
+    mod.backward_fp8 = False
+    x.requires_grad_()
+    mod(x).backward(g)
+    for got, want in ((x.grad, g.double() @ w.double()), (mod.weight.grad, g.double().t() @ x.detach().double())):
+        assert off(got.double().cpu().numpy(), want.cpu().numpy()) < 2.0 ** -8
+    if N % 16 or K % 16:                                               # the same without being asked
+        plain = [t.detach().requires_grad_() for t in (x, w, b)]
+        got = torch.autograd.grad(int8.int8_linear_train(*plain), plain, g)
+        assert torch.equal(got[0], x.grad) and torch.equal(got[1], mod.weight.grad) and torch.equal(got[2], mod.bias.grad)
+
+
+def test_empty_batch():
+    x, w, b, _ = tensors(4, 32, 48)
+    leaves = [t.requires_grad_() for t in (x[:0].detach(), w, b)]
+    y = int8.int8_linear_train(*leaves)
+    assert y.shape == (0, 32)
+    gx, gw, gb = torch.autograd.grad(y.sum(), leaves)
+    assert gx.shape == (0, 48) and not gw.any() and not gb.any()
+
+
+def test_module_and_weight_cache():
+    x, w, b, g = tensors(130, 256, 512)
+    lin = nn.Linear(512, 256, device="cuda", dtype=torch.bfloat16)
+    lin.load_state_dict({"weight": w, "bias": b})
+    mod = int8.Int8Linear.from_linear(lin)
+    assert mod.weight is lin.weight
+    x.requires_grad_()
+    y = mod(x.view(2, 65, 512))
+    y.backward(g.view(2, 65, 256))
+    want = [t.clone() for t in (y.detach(), x.grad, mod.weight.grad, mod.bias.grad)]
+    codes, scale = quant_rows(x.detach())
+    assert torch.equal(mod.forward_codes(codes, scale), want[0].view(130, 256))
+    r = seeded((130, 256), 7, torch.bfloat16)
+    assert torch.equal(mod(x.detach(), residual=r), mod.forward_codes(codes, scale, residual=r))
+    x.grad = mod.weight.grad = mod.bias.grad = None
+    with fp8_weight_cache(nn.ModuleList([mod])):
+        assert mod.weight_codes()[0].dtype == torch.int8
+        for _ in range(2):
+            x.grad = mod.weight.grad = mod.bias.grad = None
+            y = mod(x.view(2, 65, 512))
+            y.backward(g.view(2, 65, 256))
+            assert all(torch.equal(p, q) for p, q in zip((y.detach(), x.grad, mod.weight.grad, mod.bias.grad), want))
+        assert torch.equal(mod.forward_codes(codes, scale), want[0].view(130, 256))
+    with torch.autocast("cuda", dtype=torch.bfloat16), torch.no_grad():
+        assert torch.equal(mod(x.float()), want[0].view(130, 256))
+    with pytest.raises(RuntimeError, match="stale"):
+        with fp8_weight_cache(nn.ModuleList([mod])):
+            mod.weight.data += 1
+
+
+def test_training_step_in_a_graph():
+    x, w, _, g = tensors(64, 128, 256)
+    lin = int8.Int8Linear(256, 128, bias=False, device="cuda", dtype=torch.bfloat16)
+    lin.weight.data.copy_(w)
+    held = x.detach().clone().requires_grad_()
+
+    def step():
+        return torch.autograd.grad(lin(held), [held, lin.weight], g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        with torch.no_grad():
+            held.copy_(seeded((64, 256), 30 + seed, torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        own = held.detach().clone().requires_grad_()
+        y = lin(own)
+        want = torch.autograd.grad(y, [own, lin.weight], g)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
