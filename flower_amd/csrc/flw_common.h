@@ -161,6 +161,28 @@ __device__ __forceinline__ bool finite_bits(float x) {
 // integer max over it is an abs-max that propagates NaN (as torch.amax does).
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
+// A row in int8, from the bit pattern m of its largest |h|: the scale max(max|h| / 127, 1e-12) and the codes rne(h / scale). int8
+// holds no NaN: where the maximum is not finite the scale is NaN and the codes are 0.
+struct Int8Scale {
+  float scale, rcp;
+  bool finite;
+  __device__ __forceinline__ explicit Int8Scale(uint32_t m) : finite(m < 0x7F800000u) {
+    const float s = __uint_as_float(m) / 127.0f;
+    scale = finite ? (s < kEps ? kEps : s) : __uint_as_float(0x7FC00000u);
+    rcp = 1.0f / scale;
+  }
+  // Of 8 values. rne(q) lies in the low byte of q + 1.5 2^23, in two's complement.
+  __device__ __forceinline__ uint2 codes(const float* f) const {
+    uint32_t w[2] = {0, 0};
+    if (finite) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        w[e >> 2] |= (__float_as_uint(div_by_scale(f[e], scale, rcp) + 12582912.0f) & 0xFFu) << (8 * (e & 3));
+    }
+    return make_uint2(w[0], w[1]);
+  }
+};
+
 // Wave64 reductions.
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 #pragma unroll

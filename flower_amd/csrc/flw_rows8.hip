@@ -170,27 +170,24 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
 #pragma unroll
     for (int e = 0; e < 8; ++e) { const uint32_t a = abs_bits(f[i][e]); m = m > a ? m : a; }
   m = rows8_reduce<LPR>(m, red[1], [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-  const float amax = __uint_as_float(m);
-  const bool finite = m < 0x7F800000u;
-  float s = amax / (p.e4m3 ? kE4m3Max : 127.0f);
-  s = s < kEps ? kEps : s;                         // NaN stays
-  if (!p.e4m3 && !finite) s = __uint_as_float(0x7FC00000u);
+  uint8_t* dst = p.codes + row * p.cs;
+  const Int8Scale s8(m);
+  float s = s8.scale;
+  if (p.e4m3) {
+    s = __uint_as_float(m) / kE4m3Max;
+    s = s < kEps ? kEps : s;                       // NaN stays
+  }
   if (lane == 0) p.scale[row] = s;
   const float rcp = 1.0f / s;
-  uint8_t* dst = p.codes + row * p.cs;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = 8 * (lane + LPR * i);
     if (c >= cols) continue;
     uint32_t w[2] = {0, 0};
     if (!p.e4m3) {
-      if (finite) {
-        // rne(q) lies in the low byte of q + 1.5 2^23, in two's complement
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w[e >> 2] |= (__float_as_uint(div_by_scale(f[i][e], s, rcp) + 12582912.0f) & 0xFFu) << (8 * (e & 3));
-      }
-    } else if (finite) {
+      const uint2 t = s8.codes(f[i]);
+      w[0] = t.x; w[1] = t.y;
+    } else if (s8.finite) {
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {
         int t = __builtin_amdgcn_cvt_pk_fp8_f32(div_by_scale(f[i][e], s, rcp), div_by_scale(f[i][e + 1], s, rcp), 0, false);

@@ -164,6 +164,21 @@ def test_product(M, N, K):
     check_product(int8_scaled_mm(a, sa, b, one), a, sa, b, one.expand(N))
 
 
+@pytest.mark.parametrize("M,N,K", [(4096, 2304, 1296), (4100, 2312, 256), (8200, 8200, 144), (2500, 3000, 384), (4097, 2307, 272), (3000, 1280, 3392),
+                                   (5000, 1024, 128)])
+def test_large_products(M, N, K):
+    """To the bit, against sums in float64 (exact: below 2^53) on the GPU: more tiles than one a compute unit, ragged ones, outputs
+    of both sides of the size from which they pass the caches by."""
+    a, sa, b, sb = product(M, N, K)
+    v = (a.double() @ b.double().t()).float().mul_(sa[:, None]).mul_(sb).bfloat16()
+    assert torch.equal(int8_scaled_mm(a, sa, b, sb), v)
+    res = seeded((M, N), 1, torch.bfloat16)
+    assert torch.equal(int8_scaled_mm(a, sa, b, sb, residual=res), (res.float() + v.float()).bfloat16())
+    bias = seeded((N,), 2)
+    few = [0, 1, M // 2, M - 1]
+    assert torch.equal(int8_scaled_mm(a, sa, b, sb, bias=bias)[few], int8_scaled_mm(a[few], sa[few], b, sb, bias=bias))
+
+
 @pytest.mark.parametrize("M", [1, 40, 700])
 def test_product_at_the_ends_of_its_range(M):
     """The longest K that int32 holds, with every product the largest: 128 * 128 * 131071 and its negative."""
@@ -206,7 +221,8 @@ def test_a_row_alone_is_the_row_in_a_batch():
         assert torch.equal(part, whole[rows]), len(rows)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 3840, 1280), (3, 130, 17), (4, 1280, 3392), (16, 100, 31), (48, 1280, 1280), (517, 1283, 1291),
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 3840, 1280), (3, 130, 17), (4, 1280, 3392), (16, 100, 31), (2, 96, 2064), (3, 1288, 1296), (5, 64, 16),
+                                   (16, 1003, 4112), (7, 320, 8192), (1, 48, 16), (48, 1280, 1280), (517, 1283, 1291),
                                    (300, 512, 4096), (1, 64, 32768)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_linear_is_its_two_parts(M, N, K, dtype):
