@@ -42,19 +42,20 @@ struct Int8Params {
   int wide;                // N % 8 == 0, rows of y and of the residual start on 16 bytes, sb too, one a column
 };
 
-// 16 bytes at any address; 16 bytes of row p from k on, zeros past K.
+// 16 bytes at any address.
 __device__ __forceinline__ uint4 load_any16(const int8_t* p) {
   struct __attribute__((packed, aligned(1))) V { uint32_t w[4]; };
   const V v = *reinterpret_cast<const V*>(p);
   return make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
 }
-__device__ __forceinline__ uint4 load_k16(const int8_t* p, int k, int K) {
-  if (k + 16 <= K) return load_any16(p + k);
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (k + j < K) w[j >> 2] |= (uint32_t)(uint8_t)p[k + j] << (8 * (j & 3));
-  return make_uint4(w[0], w[1], w[2], w[3]);
+// v without its first s bytes, zeros behind (s >= 0).
+__device__ __forceinline__ uint4 drop_bytes(uint4 v, int s) {
+  uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
+  if (s >= 8) { lo = hi; hi = 0; }
+  const int r = 8 * (s & 7);
+  lo = s >= 16 ? 0 : r ? lo >> r | hi << (64 - r) : lo;
+  hi >>= r;
+  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
 __device__ __forceinline__ float int8_bias(const Int8Params& p, int n) {
@@ -75,76 +76,6 @@ __device__ __forceinline__ void each_up(F f) {            // f(0), ..., f(N - 1)
 
 // One output before the residual. The same operations in every kernel, so that all give the same bits.
 __device__ __forceinline__ float int8_value(int acc, float sa, float sb, float bias) { return fmaf((float)acc * sa, sb, bias); }
-
-// Any sizes and alignments: tiles of 64 (n) x 64 (m), 2 x 2 waves, 128 K bytes a stage through registers, three stages of them
-// under way, into two LDS buffers ([517, 1283] at K = 1291: ANYUS us; ANYOLD with one stage under way).
-constexpr int kIK = 128, kAnyAhead = 3;
-
-__global__ __launch_bounds__(256) void int8_any_kernel(Int8Params p) {
-  __shared__ __align__(16) uint8_t lds[2][2][64 * kIK];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wn = wave & 1, wm = wave >> 1;
-  const int n0 = (int)(blockIdx.x % p.tiles_n) * 64, m0 = (int)(blockIdx.x / p.tiles_n) * 64;
-  const int c16 = 16 * (tid & 7), stages = (p.K + kIK - 1) / kIK;
-  const int8_t *gb[2], *ga[2];                    // this thread's rows tid / 8 and 32 + tid / 8 (past the last: that one again)
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    gb[j] = p.b + (int64_t)min(n0 + 32 * j + (tid >> 3), p.N - 1) * p.bs;
-    ga[j] = p.a + (int64_t)min(m0 + 32 * j + (tid >> 3), p.M - 1) * p.as;
-  }
-  uint4 rb[kAnyAhead][2], ra[kAnyAhead][2];
-  auto load = [&](int s, auto uc) __attribute__((always_inline)) {
-    constexpr int u = decltype(uc)::value;
-    const int k = s * kIK + c16;
-    if ((s + 1) * kIK <= p.K) {                   // uniform
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        rb[u][j] = load_any16(gb[j] + k);
-        ra[u][j] = load_any16(ga[j] + k);
-      }
-    } else if (s < stages) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        rb[u][j] = load_k16(gb[j], k, p.K);
-        ra[u][j] = load_k16(ga[j], k, p.K);
-      }
-    }
-  };
-  v16i acc = {};
-  each_up<kAnyAhead>([&](auto u) __attribute__((always_inline)) { load(decltype(u)::value, u); });
-  for (int s0 = 0; s0 < stages; s0 += kAnyAhead)
-    each_up<kAnyAhead>([&](auto uc) __attribute__((always_inline)) {
-      constexpr int u = decltype(uc)::value;
-      const int s = s0 + u, buf = s & 1;
-      if (s < stages) {                           // uniform
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int off = swz(32 * j + (tid >> 3), tid & 7);
-          *reinterpret_cast<uint4*>(&lds[buf][0][off]) = rb[u][j];
-          *reinterpret_cast<uint4*>(&lds[buf][1][off]) = ra[u][j];
-        }
-        __syncthreads();                          // stage s is there, and every wave is done with stage s - 1
-        load(s + kAnyAhead, uc);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {             // 16-byte chunks 4 (q / 2) + 2 (lane / 32) + q % 2 of the row
-          const int c = 4 * (q >> 1) + 2 * (lane >> 5) + (q & 1);
-          const v4i fb = *reinterpret_cast<const v4i*>(&lds[buf][0][swz(32 * wn + (lane & 31), c)]);
-          const v4i fa = *reinterpret_cast<const v4i*>(&lds[buf][1][swz(32 * wm + (lane & 31), c)]);
-          acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb, fa, acc, 0, 0, 0);
-        }
-      }
-    });
-  const int m = m0 + 32 * wm + (lane & 31);
-  if (m >= p.M) return;
-  const float sa = p.sa[(int64_t)m * p.sa_step];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int n = n0 + 32 * wn + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-    if (n >= p.N) continue;
-    float v = int8_value(acc[e], sa, p.sb[(int64_t)n * p.sb_step], int8_bias(p, n));
-    if (p.res) v = round_bf16(v) + bf16_to_f32(p.res[m * p.rs + n]);
-    p.y[m * p.ys + n] = (uint16_t)f32_to_bf16_bits(v);
-  }
-}
 
 // ---------------------------------------------------------------- tiles through LDS
 //
@@ -256,6 +187,70 @@ __device__ __forceinline__ void int8_epilogue(const Int8Params& p, const v16i (&
     const uint4 o = *reinterpret_cast<const uint4*>(lds + r * ROWB + 16 * (ch ^ (r & (CPR - 1))));
     int8_store8(p, m, n, o);
   }
+}
+
+// Any sizes and alignments: tiles of 64 (n) x 64 (m), 2 x 2 waves, 128 K bytes a stage through registers, three stages of them
+// under way, into two LDS buffers ([517, 1283] at K = 1291: ANYUS us; 22 with one stage under way). Behind K a load takes the row's
+// last 16 bytes, and what it should not have is dropped on the way to LDS: no load stands in a branch. SHORT: K < 16.
+constexpr int kAnyAhead = 3;
+
+template <bool SHORT>
+__global__ __launch_bounds__(256) void int8_any_kernel(Int8Params p) {
+  __shared__ __align__(16) uint8_t lds[2][2][64 * 128];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wn = wave & 1, wm = wave >> 1;
+  const int n0 = (int)(blockIdx.x % p.tiles_n) * 64, m0 = (int)(blockIdx.x / p.tiles_n) * 64;
+  const int c16 = 16 * (tid & 7), stages = (p.K + 127) >> 7;
+  const int8_t* g[2][2];                          // b's and a's rows tid / 8 and 32 + tid / 8 (past the last: that one again)
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    g[0][j] = p.b + (int64_t)min(n0 + 32 * j + (tid >> 3), p.N - 1) * p.bs;
+    g[1][j] = p.a + (int64_t)min(m0 + 32 * j + (tid >> 3), p.M - 1) * p.as;
+  }
+  uint4 v[kAnyAhead][2][2];
+  auto load = [&](int s, auto uc) __attribute__((always_inline)) {
+    constexpr int u = decltype(uc)::value;
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (SHORT) {
+          uint8_t byte[16] = {};
+          for (int k = 0; k < p.K; ++k)
+            if (c16 == 0) byte[k] = (uint8_t)g[o][j][k];
+          v[u][o][j] = __builtin_bit_cast(uint4, byte);
+        } else {
+          v[u][o][j] = load_any16(g[o][j] + min(128 * s + c16, p.K - 16));
+        }
+      }
+  };
+  v16i acc[2] = {};
+  each_up<kAnyAhead>([&](auto u) __attribute__((always_inline)) { load(decltype(u)::value, u); });
+  for (int s0 = 0; s0 < stages; s0 += kAnyAhead)
+    each_up<kAnyAhead>([&](auto uc) __attribute__((always_inline)) {
+      constexpr int u = decltype(uc)::value;
+      const int s = s0 + u, buf = s & 1;
+      if (s < stages) {                           // uniform
+        if (!SHORT && s == stages - 1) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[u][j >> 1][j & 1] = drop_bytes(v[u][j >> 1][j & 1], max(128 * s + c16 - (p.K - 16), 0));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint4*>(&lds[buf][j >> 1][swz(32 * (j & 1) + (tid >> 3), tid & 7)]) = v[u][j >> 1][j & 1];
+        __syncthreads();                          // stage s is there, and every wave is done with stage s - 1
+        load(s + kAnyAhead, uc);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {             // 16-byte chunks 4 (q / 2) + 2 (lane / 32) + q % 2 of the row
+          const int c = 4 * (q >> 1) + 2 * (lane >> 5) + (q & 1);
+          const v4i fb = *reinterpret_cast<const v4i*>(&lds[buf][0][swz(32 * wn + (lane & 31), c)]);
+          const v4i fa = *reinterpret_cast<const v4i*>(&lds[buf][1][swz(32 * wm + (lane & 31), c)]);
+          acc[q & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb, fa, acc[q & 1], 0, 0, 0);
+        }
+      }
+    });
+  __syncthreads();                                // the epilogue overwrites the stages
+  v16i sum[1][1] = {acc[0] + acc[1]};
+  int8_epilogue<2, 2, 1, 1>(p, sum, &lds[0][0][0], m0, n0, wave, lane);
 }
 
 template <int WN, int WM, int TN, int TM, int NST, bool TAIL>
@@ -785,7 +780,8 @@ static int int8_mm(Int8Params p, int64_t M, int64_t N, int64_t K, int64_t sa_cou
   }
   p.wide = N % 8 == 0 && p.sb_step == 1 && (uintptr_t)p.sb % 16 == 0 && on16(p.y, 2 * p.ys, M) &&
            (p.res == nullptr || on16(p.res, 2 * p.rs, M));
-  const Int8Kernel k = vector ? kernel_of(p) : Int8Kernel{reinterpret_cast<const void*>(&int8_any_kernel), 64, 64, 256, false};
+  const Int8Kernel k = vector ? kernel_of(p) : Int8Kernel{K < 16 ? reinterpret_cast<const void*>(&int8_any_kernel<true>) : reinterpret_cast<const void*>(&int8_any_kernel<false>),
+                                                       64, 64, 256, false};
   const int64_t tiles_n = (N + k.bn - 1) / k.bn, tiles_m = (M + k.bm - 1) / k.bm;
   FLW_REQUIRE(tiles_n * tiles_m <= 0x3FFFFFFFll, FLW_E_UNSUPPORTED, "too many output tiles");
   p.tiles_n = (int)tiles_n;

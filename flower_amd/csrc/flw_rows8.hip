@@ -71,6 +71,14 @@ __device__ __forceinline__ void rows8_store(T* row, int c, int cols, const float
   } else if constexpr (ALIGNED) {
     *reinterpret_cast<float4*>(row + c) = make_float4(f[0], f[1], f[2], f[3]);
     *reinterpret_cast<float4*>(row + c + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  } else if (c + 8 <= cols) {
+    struct __attribute__((packed, aligned(sizeof(T)))) V { uint32_t w[2 * sizeof(T)]; } v;
+#pragma unroll
+    for (int j = 0; j < 8; j += 4 / sizeof(T)) {
+      if constexpr (sizeof(T) == 2) v.w[j / 2] = bf16x2_rne(f[j], f[j + 1]);
+      else v.w[j] = __float_as_uint(f[j]);
+    }
+    *reinterpret_cast<V*>(row + c) = v;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -133,7 +141,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
         rows8_store<T, ALIGNED>(static_cast<T*>(p.sum) + row * p.ss, c, cols, f[i]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] / (1.0f + expf(-f[i][e])) * g[i][e];
+        for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * __builtin_amdgcn_rcpf(1.0f + expf(-f[i][e])) * g[i][e];
       }
     }
   }
@@ -162,7 +170,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] = 0.5f * f[i][e] * (1.0f + erff(f[i][e] * 0.70710678118654752f));
+      for (int e = 0; e < 8; ++e) f[i][e] = gelu_as(f[i][e]);
   }
   uint32_t m = 0;                                  // |h| as bit patterns: NaN above infinity above the rest
 #pragma unroll
@@ -200,6 +208,9 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
     }
     if constexpr (ALIGNED) {
       *reinterpret_cast<uint2*>(dst + c) = make_uint2(w[0], w[1]);
+    } else if (c + 8 <= cols) {
+      struct __attribute__((packed, aligned(1))) V { uint32_t w[2]; };
+      *reinterpret_cast<V*>(dst + c) = V{w[0], w[1]};
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -251,8 +262,10 @@ static int rows8(Rows8Params p, int dtype, int64_t cols, int weight_dtype, int c
   p.e4m3 = code_type == FLW_E4M3;
   const bool aligned = cols % 8 == 0 && rows16(p.x, p.xs, size) && rows16(p.b, p.bs, size) && rows16(p.sum, p.ss, size) &&
                        rows16(p.w, 0, 4) && (uintptr_t)p.codes % 8 == 0 && p.cs % 8 == 0;
-  // The fewest lanes whose four chunks hold the row.
-  const int lpr = cols <= 2048 ? 64 : cols <= 8192 ? 256 : 1024;
+  // The fewest lanes whose four chunks hold the row, and more for few rows, where a row's latency counts and no lane is missed
+  // elsewhere (us, on 64 / 256 lanes: addnorm [1, 1280] 4.4 / 3.1, [1024, 1280] 5.6 / 4.4, [8192, 1280] 17.6 / 17.9, norm there
+  // 10.2 / 12.6; on 256 / 1024: addnorm [24, 3392] 4.3 / 3.7, [1024, 4096] 9.3 / 10.2).
+  const int lpr = cols <= 512 || (cols <= 2048 && p.rows > 2048) ? 64 : cols <= 2048 || (cols <= 8192 && p.rows > 128) ? 256 : 1024;
   const int nc = (int)((cols + 8 * lpr - 1) / (8 * lpr));
   const void* kernel = dtype == FLW_F32 ? (aligned ? rows8_of<float, OP, true>(lpr, nc) : rows8_of<float, OP, false>(lpr, nc))
                                         : (aligned ? rows8_of<uint16_t, OP, true>(lpr, nc) : rows8_of<uint16_t, OP, false>(lpr, nc));
