@@ -89,6 +89,12 @@ __device__ __forceinline__ void rows8_store(T* row, int c, int cols, const float
   }
 }
 
+// x / (1 + exp(-x)), the quotient by a reciprocal and one correction (the denominator within what fp32 can invert: x / d is 0 there).
+__device__ __forceinline__ float silu(float x) {
+  const float d = fminf(1.0f + expf(-x), 1e38f), r = __builtin_amdgcn_rcpf(d), q = x * r;
+  return fmaf(fmaf(-q, d, x), r, q);
+}
+
 // One value of every lane of a row, combined over the row's LPR lanes (the same bits in all of them).
 template <int LPR, typename F>
 __device__ __forceinline__ uint32_t rows8_reduce(uint32_t v, uint32_t* red, F f) {
@@ -141,7 +147,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
         rows8_store<T, ALIGNED>(static_cast<T*>(p.sum) + row * p.ss, c, cols, f[i]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * __builtin_amdgcn_rcpf(1.0f + expf(-f[i][e])) * g[i][e];
+        for (int e = 0; e < 8; ++e) f[i][e] = silu(f[i][e]) * g[i][e];
       }
     }
   }
@@ -170,7 +176,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] = gelu_as(f[i][e]);
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.5f * f[i][e] * (1.0f + erff(f[i][e] * 0.70710678118654752f));
   }
   uint32_t m = 0;                                  // |h| as bit patterns: NaN above infinity above the rest
 #pragma unroll
@@ -217,6 +223,55 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
         if (c + e < cols) dst[c + e] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
     }
   }
+}
+
+// Column sums of bf16 rows (a bias's gradient), in two passes of a fixed order: each workgroup sums 512 columns (8 a lane) of
+// kSumRows rows, its four waves every fourth row, into part [chunks][cols]; then the chunks of each column are summed.
+constexpr int kSumRows = 128;
+
+template <bool ALIGNED>
+__global__ __launch_bounds__(256) void col_sum_kernel(const uint16_t* __restrict__ x, int64_t rows, int cols, int64_t xs,
+                                                      float* __restrict__ part) {
+  __shared__ float fold[3][512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 512 + 8 * lane;
+  const int64_t r1 = min(rows, (int64_t)(blockIdx.y + 1) * kSumRows);
+  float acc[8] = {};
+  if (c < cols) {
+#pragma unroll 4
+    for (int64_t r = (int64_t)blockIdx.y * kSumRows + wave; r < r1; r += 4) {
+      float f[8];
+      rows8_load<uint16_t, ALIGNED>(x + r * xs, c, cols, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += f[e];
+    }
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) fold[wave - 1][64 * e + lane] = acc[e];
+  }
+  __syncthreads();
+  if (wave > 0 || c >= cols) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (c + e < cols)
+      part[(int64_t)blockIdx.y * cols + c + e] = ((acc[e] + fold[0][64 * e + lane]) + fold[1][64 * e + lane]) + fold[2][64 * e + lane];
+}
+
+// 16 columns a workgroup, 16 slices of the chunks each.
+__global__ __launch_bounds__(256) void col_sum_fold_kernel(const float* __restrict__ part, int chunks, int cols, void* __restrict__ out,
+                                                           int out32) {
+  __shared__ float red[16][17];
+  const int cl = threadIdx.x & 15, s = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  float a = 0.0f;
+  if (c < cols)
+    for (int k = s; k < chunks; k += 16) a += part[(int64_t)k * cols + c];
+  red[s][cl] = a;
+  __syncthreads();
+  if (s > 0 || c >= cols) return;
+#pragma unroll
+  for (int j = 1; j < 16; ++j) a += red[j][cl];
+  if (out32) static_cast<float*>(out)[c] = a;
+  else static_cast<uint16_t*>(out)[c] = (uint16_t)f32_to_bf16_bits(a);
 }
 
 template <typename T, int OP, bool ALIGNED>
@@ -312,4 +367,33 @@ extern "C" int flw_rows8_swiglu(const void* gate, const void* up, int dtype, int
   p.x = gate; p.rows = rows; p.xs = gate_row_stride; p.codes = static_cast<uint8_t*>(codes); p.cs = codes_row_stride; p.scale = scale;
   p.b = up; p.bs = up_row_stride;
   return rows8<kRows8Swiglu>(p, dtype, cols, dtype, code_type, stream, "flw_rows8_swiglu");
+}
+
+static int64_t sum_chunks(int64_t rows) { return (rows + kSumRows - 1) / kSumRows; }
+
+extern "C" size_t flw_col_sum_workspace_bytes(int64_t rows, int64_t cols) {
+  return rows <= 0 || cols <= 0 ? 0 : (size_t)(sum_chunks(rows) * cols * 4);
+}
+
+extern "C" int flw_col_sum(const void* x, int64_t rows, int64_t cols, int64_t x_row_stride, void* out, int out_dtype, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  FLW_REQUIRE(rows > 0 && cols > 0, FLW_E_INVALID, "empty or negative shape (%lld, %lld)", (long long)rows, (long long)cols);
+  FLW_REQUIRE(cols <= 0x7FFFFE00ll && sum_chunks(rows) <= 65535, FLW_E_UNSUPPORTED, "too many rows or columns");
+  FLW_REQUIRE(out_dtype == FLW_F32 || out_dtype == FLW_BF16, FLW_E_UNSUPPORTED, "dtype %d not supported (f32=0, bf16=1)", out_dtype);
+  FLW_REQUIRE(rows_ok(x, x_row_stride, cols, 2) && rows_ok(out, cols, cols, out_dtype == FLW_F32 ? 4 : 2), FLW_E_INVALID,
+              "null or misaligned pointer, or a row stride below the row");
+  const size_t need = flw_col_sum_workspace_bytes(rows, cols);
+  FLW_REQUIRE(workspace_bytes >= need && workspace != nullptr && (uintptr_t)workspace % 16 == 0, FLW_E_WORKSPACE,
+              "workspace needs %zu bytes (16-byte aligned), got %zu", need, workspace_bytes);
+  const int chunks = (int)sum_chunks(rows);
+  const bool aligned = cols % 8 == 0 && rows16(x, x_row_stride, 2);
+  const Timer tm = take_timer();
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  float* part = static_cast<float*>(workspace);
+  (void)launch_args(aligned ? reinterpret_cast<const void*>(&col_sum_kernel<true>) : reinterpret_cast<const void*>(&col_sum_kernel<false>),
+                    dim3((unsigned)((cols + 511) / 512), (unsigned)chunks), dim3(256), 0, s, tm.start, nullptr,
+                    static_cast<const uint16_t*>(x), rows, (int)cols, x_row_stride, part);
+  (void)launch_args(reinterpret_cast<const void*>(&col_sum_fold_kernel), dim3((unsigned)((cols + 15) / 16)), dim3(256), 0, s, nullptr,
+                    tm.stop, static_cast<const float*>(part), chunks, (int)cols, out, (int)(out_dtype == FLW_F32));
+  return check_launch("flw_col_sum");
 }

@@ -934,6 +934,41 @@ Tensor int8_linear(const Tensor& x0, const Tensor& b0, const Tensor& b_scale, co
   return p.y;
 }
 
+// The gradients of y = x W^T (+ bias) straight through its quantisers, from g = dy: (dx, dW, db), each when asked for. The products
+// are the e4m3 ones of the rowwise recipe: g by rows with W by columns (w_cols: its codes transposed and scales, made here if not
+// given), and g by columns with x by columns, the token axis padded with zeros to a multiple of 128. N and K are multiples of 16.
+// All of it in one call: a small step's fourteen launches take less time than as many calls from Python.
+std::tuple<OptTensor, OptTensor, OptTensor> int8_linear_bwd(const Tensor& g0, const Tensor& x0, const Tensor& weight,
+                                                            const std::optional<std::pair<Tensor, Tensor>>& w_cols, bool need_x,
+                                                            bool need_w, const std::optional<at::ScalarType>& bias_dtype, int64_t stream) {
+  c10::DeviceGuard guard(x0.device());
+  const int64_t N = weight.size(0), K = weight.size(1);
+  const Tensor g = rows16(g0.reshape({-1, N}).to(at::kBFloat16));
+  const int64_t M = g.size(0), ld = (M + 127) / 128 * 128;
+  OptTensor dx, dw, db;
+  if (need_x) {
+    Rows8 rows(g, true);
+    check(flw_rows8(g.data_ptr(), FLW_BF16, M, N, M > 1 ? g.stride(0) : N, FLW_E4M3, rows.codes.data_ptr(), N, f32(rows.scale),
+                    str(stream)),
+          "int8 linear backward");
+    const auto cols = w_cols ? std::make_tuple(w_cols->first, w_cols->second) : quant_cols(rows16(weight), true, N, stream);
+    dx = scaled_mm(rows.codes, rows.scale, std::get<0>(cols), std::get<1>(cols), std::nullopt, true, stream);
+  }
+  if (need_w) {
+    const auto [g8, gs] = quant_cols(g, true, ld, stream);
+    const auto [x8, xs] = quant_cols(rows16(x0.reshape({-1, K})), true, ld, stream);
+    dw = scaled_mm(g8, gs, x8, xs, std::nullopt, true, stream);
+  }
+  if (bias_dtype) {
+    db = empty(g, {N}, *bias_dtype == at::kFloat ? at::kFloat : at::kBFloat16);
+    const Tensor ws = workspace(g, flw_col_sum_workspace_bytes(M, N));
+    check(flw_col_sum(g.data_ptr(), M, N, M > 1 ? g.stride(0) : N, db->data_ptr(), dtype_code(*db), ws.data_ptr(), (size_t)ws.numel(),
+                      str(stream)),
+          "int8 linear backward");
+  }
+  return {dx, dw, db};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -980,4 +1015,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("act_quant", &act_quant, nogil());
   m.def("int8_scaled_mm", &int8_scaled_mm, nogil());
   m.def("int8_linear", &int8_linear, nogil());
+  m.def("int8_linear_bwd", &int8_linear_bwd, nogil());
 }

@@ -15,7 +15,7 @@ import torch.nn as nn
 
 from . import _lib
 from .kernels.int8 import int8_scaled_mm, quant_rows
-from .precision import Fp8Linear, fp8_linear_backward, fp8_module_filter, quantize_weight_cols
+from .precision import Fp8Linear, fp8_module_filter, quantize_weight_cols
 
 
 def quantize_weight_int8(weight: torch.Tensor):
@@ -25,41 +25,44 @@ def quantize_weight_int8(weight: torch.Tensor):
 
 class _Int8LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, w8, w_scale, mod):
+    def forward(ctx, x, weight, bias, residual, codes, mod):
+        native, stream = _lib.native(), _lib.stream_or_none(x)
+        w8, w_scale = native.quant_rows8(weight, False, stream) if codes is None else codes
         ctx.save_for_backward(x, weight)
         ctx.mod, ctx.bias_dtype = mod, None if bias is None else bias.dtype
-        return _lib.native().int8_linear(x, w8, w_scale, bias, residual, _lib.stream_or_none(x))
+        return native.int8_linear(x, w8, w_scale, bias, residual, stream)
 
     @staticmethod
     def backward(ctx, g):
         x, weight = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        N, K = weight.shape
-        g2, x2 = g.reshape(-1, N), x.reshape(-1, K)
+        (N, K), mod = weight.shape, ctx.mod
         gx = gw = gb = None
-        if g2.shape[0] == 0:
+        if g.numel() == 0:
             gx = torch.zeros_like(x) if need_x else None
             gw = torch.zeros_like(weight) if need_w else None
-        # The e4m3 products take widths in whole 16-byte rows; others, and a module that asks for it, run in bf16.
-        elif (ctx.mod is None or ctx.mod.backward_fp8) and N % 16 == 0 and K % 16 == 0:
-            cols = ctx.mod.weight_col_codes if ctx.mod is not None else lambda: quantize_weight_cols(weight, "rowwise")
-            gx, gw = fp8_linear_backward(g2, x2, cols, "rowwise", need_x, need_w)
-        else:
+            gb = weight.new_zeros(N, dtype=ctx.bias_dtype) if need_b else None
+            return gx, gw, gb, (g if need_r else None), None, None
+        # The e4m3 products take widths in whole 16-byte rows and the types that the casts read; others, and a module that asks
+        # for it, run in bf16.
+        fp8 = N % 16 == 0 and K % 16 == 0 and (mod is None or mod.backward_fp8)
+        cols = mod.weight_col_codes() if fp8 and need_x and mod is not None else None
+        gx, gw, gb = _lib.native().int8_linear_bwd(g, x, weight, cols, fp8 and need_x, fp8 and need_w, ctx.bias_dtype if need_b else None,
+                                                   _lib.stream_or_none(x))
+        if not fp8:
+            g2 = g.reshape(-1, N)
             gx = g2 @ weight.to(g2.dtype) if need_x else None
-            gw = g2.t() @ x2.to(g2.dtype) if need_w else None
-        gx = gx.reshape(x.shape).to(x.dtype) if gx is not None else None
+            gw = g2.t() @ x.reshape(-1, K).to(g2.dtype) if need_w else None
+        gx = gx.view(x.shape).to(x.dtype) if gx is not None else None
         gw = gw.to(weight.dtype) if gw is not None else None
-        if need_b:
-            gb = g2.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
-        return gx, gw, gb, (g if need_r else None), None, None, None
+        return gx, gw, gb, (g if need_r else None), None, None
 
 
 def int8_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                       residual: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight^T + bias``, plus ``residual``, in int8: both operands quantised now, a scale a token and a channel; bf16 out.
-    x (.., K), weight (N, K) bf16 or fp32. Differentiable, as ``Int8Linear`` is."""
-    w8, w_scale = quantize_weight_int8(weight)
-    return _Int8LinearFn.apply(x, weight, bias, residual, w8, w_scale, None)
+    x (.., K), weight (N, K) and bias (N,) bf16 or fp32, residual bf16. Differentiable, as ``Int8Linear`` is."""
+    return _Int8LinearFn.apply(x, weight, bias, residual, None, None)
 
 
 class Int8Linear(Fp8Linear):
@@ -95,11 +98,11 @@ class Int8Linear(Fp8Linear):
     def forward_with(self, x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, x_amax=None, residual=None,
                      w8t=None) -> torch.Tensor:
         """x_amax and w8t are of the tensorwise recipe: not used."""
-        if torch.is_autocast_enabled():
-            x = x.to(torch.get_autocast_gpu_dtype())
+        if torch.is_autocast_enabled("cuda"):
+            x = x.to(torch.get_autocast_dtype("cuda"))
         elif x.dtype not in (torch.bfloat16, torch.float32):
             x = x.to(torch.bfloat16)
-        return _Int8LinearFn.apply(x, self.weight, self.bias, residual, w8, w_scale, self)
+        return _Int8LinearFn.apply(x, self.weight, self.bias, residual, (w8, w_scale), self)
 
     def forward(self, x: torch.Tensor, x_amax=None, residual=None) -> torch.Tensor:
         return self.forward_with(x, *self.weight_codes(), residual=residual)

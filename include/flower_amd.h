@@ -645,6 +645,12 @@ int flw_rows8_gelu(const void* x, int dtype, int64_t rows, int64_t cols, int64_t
 int flw_rows8_swiglu(const void* gate, const void* up, int dtype, int64_t rows, int64_t cols, int64_t gate_row_stride,
                      int64_t up_row_stride, int code_type, void* codes, int64_t codes_row_stride, float* scale, void* stream);
 
+/* Column sums of bf16 rows x [rows, cols] (a bias's gradient) in fp32, in a fixed order, rounded once to out [cols], fp32 or bf16
+ * (out_dtype). Rows of any alignment. workspace: flw_col_sum_workspace_bytes(rows, cols), 16-byte aligned. */
+size_t flw_col_sum_workspace_bytes(int64_t rows, int64_t cols);
+int flw_col_sum(const void* x, int64_t rows, int64_t cols, int64_t x_row_stride, void* out, int out_dtype, void* workspace,
+                size_t workspace_bytes, void* stream);
+
 /* y[M, N] (bf16) = (a[M, K] . b[N, K]^T) * a_scale[m] * b_scale[n] + bias[n] of int8 matrices, or bf16(residual + bf16(that)):
  * the integer form of flw_fp8_scaled_mm (torch._scaled_mm, flower/models/base.py:919-923). The sums are exact in int32
  * (K <= 131071), the result does not depend on how the work is cut. Scale counts: M or 1, and N or 1. bias: NULL, fp32 or
