@@ -404,7 +404,10 @@ class CausalSelfAttention(nn.Module):
             if self.fp8_attention_sim:
                 q, k, v = _fake_quant_e4m3(q), _fake_quant_e4m3(k), _fake_quant_e4m3(v)
             return q, k, v
-        y = self.qkv(x)
+        return self.heads(self.qkv(x))
+
+    def heads(self, y: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """``qkv_heads`` behind its projection: y (B, T, 3 d) split, normed and turned."""
         if self.rope.plain and y.is_cuda and y.dtype == torch.bfloat16 and self.head_dim in (32, 64, 128):
             cos, sin = self.rope.tables(y.shape[1], y.dtype, y.device)
             eps = self.qk_norm.eps if self.qk_norm is not None else 0.0
@@ -450,10 +453,13 @@ class CausalSelfAttention(nn.Module):
             if self._needs_grad(x):
                 return self._forward_fp8_train(x)
             return self._forward_fp8(x, trace) if self.rope.plain else self.forward_unfused(x)
-        q, k, v = self.qkv_heads(x)
+        return self.out(self.attend(*self.qkv_heads(x)))
+
+    def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """The bf16 route's attention of the heads, (B, T, d) as ``out`` takes it."""
         # token-major O: the transpose back to [B, T, H D] rows below is a view, in both directions
-        out = swa_attention(q, k, v, self._window(x.shape[1]), token_major=q.dtype == torch.bfloat16)
-        return self.out(out.transpose(1, 2).reshape(x.shape))
+        out = swa_attention(q, k, v, self._window(q.shape[2]), token_major=q.dtype == torch.bfloat16)
+        return out.transpose(1, 2).reshape(q.shape[0], q.shape[2], self.num_heads * self.head_dim)
 
     def _forward_fp8(self, x: torch.Tensor, trace: dict | None = None) -> torch.Tensor:
         """qkv -> fused QK-norm + RoPE + e4m3 quantisation -> FP8 SWA -> out. ``trace`` (a dict,
@@ -498,19 +504,28 @@ class CausalSelfAttention(nn.Module):
         before an e4m3 cache's cast). Padding tokens' rows then hold no meaning (else: what ``out`` makes of zeros), and
         their x must be finite.
         """
+        self._check_cached(x, cache)
+        return self.out(self.attend_cached(self.qkv(x), cache, layer, prompt=prompt))
+
+    def _check_cached(self, x: torch.Tensor, cache) -> None:
         if x.dim() != 3 or x.shape[0] != cache.sequences:
             raise ValueError(f"x must be ({cache.sequences}, T, d), got {tuple(x.shape)}")
         if self.fp8_attention_sim:
             raise ValueError("fp8_attention_sim takes its scales from whole sequences: it has no cached form")
         if cache.window is not None and (self.local_window is None or self.local_window > cache.window):
             raise ValueError(f"the cache keeps a window of {cache.window} positions, this layer sees {self.local_window}")
-        q, k, v = (self._split(t) for t in self.qkv(x).chunk(3, dim=-1))
+
+    @torch.no_grad()
+    def attend_cached(self, y: torch.Tensor, cache, layer: int, *, prompt: bool = False) -> torch.Tensor:
+        """``forward_cached`` between its projections: from y (B, T, 3 d), what ``qkv`` gives, to the (B, T, d) that ``out`` takes."""
+        self._check_cached(y, cache)
+        q, k, v = (self._split(t) for t in y.chunk(3, dim=-1))
         cos, sin = self.rope.pair_tables(cache.max_len, q.dtype, q.device)
         how = dict(cos=cos, sin=sin, layout=self.rope.layout, norm_eps=self.qk_norm.eps if self.qk_norm is not None else None)
         if prompt:
             q, k = cache.append(layer, q, k, v, return_k=True, **how)
-            out = swa_attention(q, k, v.contiguous(), self._window(x.shape[1]), token_major=True)
+            out = swa_attention(q, k, v.contiguous(), self._window(y.shape[1]), token_major=True)
         else:
             q = cache.append(layer, q, k, v, **how)
             out = cache.attend(layer, q, window=self.local_window)
-        return self.out(out.transpose(1, 2).reshape(x.shape))
+        return out.transpose(1, 2).reshape(*y.shape[:2], self.num_heads * self.head_dim)

@@ -38,6 +38,7 @@ from . import _lib
 from .attention import CausalSelfAttention
 from .kernels.fp8_swa_attention import (fp8_swa_attention_forward, fp8_swa_attention_from_codes,
                                         qk_norm_rope_quant_e4m3)
+from .kernels.int8 import gelu_quant, rms_norm_quant, swiglu_quant
 from .precision import Fp8Linear
 
 
@@ -469,12 +470,26 @@ class FeedForward(nn.Module):
                 out = self.down(torch.nn.functional.silu(gate) * up)
         return out if residual is None else residual + out
 
+    def linears(self):
+        return (self.net[0], self.net[-1]) if self.activation == "gelu" else (self.gate, self.up, self.down)
+
+    @torch.no_grad()
+    def forward_codes(self, codes: torch.Tensor, scale: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """``forward`` of Int8Linears for an input in int8 (codes and a scale a row): the activation goes straight into the last
+        linear's int8 rows. Forward-only."""
+        *first, last = self.linears()
+        hidden = [m.forward_codes(codes, scale) for m in first]
+        return last.forward_codes(*(gelu_quant if self.activation == "gelu" else swiglu_quant)(*hidden), residual=residual)
+
 
 class TransformerBlock(nn.Module):
     """base.py:698-722 for training: ``x + attn(ln1(x))``, then ``+ ff(ln2(x))``, returning
     ``(x, memory)`` as the reference's block does. The attention is ``CausalSelfAttention`` (the
     HIP bf16 sliding-window kernels, or the FP8 route with ``attn_precision: "fp8"``) with the
-    config's window; RMSNorm norms (``norm_type: rmsnorm``, the 450M configs' choice)."""
+    config's window; RMSNorm norms (``norm_type: rmsnorm``, the 450M configs' choice).
+
+    With every Linear an ``Int8Linear`` (``convert_model_to_int8``) and no gradient to take, the norms and the activation are
+    written as the next linear's int8 rows (``_forward_int8``): a call in 8 bits end to end but for the attention."""
 
     def __init__(self, config) -> None:
         super().__init__()
@@ -485,8 +500,26 @@ class TransformerBlock(nn.Module):
         self.ln2 = RMSNorm(config.d_model)
         self.ff = FeedForward(config)
 
+    def _int8_ok(self, x: torch.Tensor) -> bool:
+        from .int8 import Int8Linear
+        return (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 3 and x.numel() > 0 and not torch.is_grad_enabled()
+                and not torch.is_autocast_enabled("cuda") and x.shape[-1] <= 32768 and self.ff.linears()[-1].in_features <= 32768
+                and all(w.dtype in (torch.bfloat16, torch.float32) for w in (self.ln1.weight, self.ln2.weight))
+                and all(type(m) is Int8Linear for m in (self.attn.qkv, self.attn.out, *self.ff.linears())))
+
+    def _forward_int8(self, x: torch.Tensor, attend) -> torch.Tensor:
+        """The block with int8 linears; attend: from the qkv projection to what ``out`` takes. The norms' outputs stay in fp32 up to
+        their codes, where the module-by-module route rounds them to bf16 in between."""
+        attn = self.attn
+        codes, scale = rms_norm_quant(x, self.ln1.weight, self.ln1.eps)
+        a = attn.out(attend(attn.qkv.forward_codes(codes, scale)))
+        codes, scale, x = rms_norm_quant(x, self.ln2.weight, self.ln2.eps, residual=a)
+        return self.ff.forward_codes(codes, scale, residual=x)
+
     def forward(self, x: torch.Tensor, memory: torch.Tensor | None = None):
         d = x.shape[-1]
+        if self.attn.attn_precision == "bf16" and self._int8_ok(x):
+            return self._forward_int8(x, lambda y: self.attn.attend(*self.attn.heads(y))), memory
         if d % 8 == 0 and d <= 8192 and x.numel() > 0 and _hip_rows_ok(x, self.ln1.weight, self.ln2.weight):
             # bf16 on the GPU: ln1 hands x on as the residual stream and ln2 takes the first
             # residual add into its pass, so the norms' backward passes also add the residual
@@ -502,6 +535,8 @@ class TransformerBlock(nn.Module):
     def forward_cached(self, x: torch.Tensor, cache, layer: int, *, prompt: bool = False) -> torch.Tensor:
         """The new tokens x (B, T, d) through the block, their keys and values into layer ``layer`` of ``cache``
         (``CausalSelfAttention.forward_cached``). Forward-only."""
+        if self._int8_ok(x) and x.shape[0] == cache.sequences:
+            return self._forward_int8(x, lambda y: self.attn.attend_cached(y, cache, layer, prompt=prompt))
         a = self.attn.forward_cached(self.ln1(x), cache, layer, prompt=prompt)
         d = x.shape[-1]
         if d % 8 == 0 and d <= 8192 and x.numel() > 0 and _hip_rows_ok(x, a, self.ln2.weight):
