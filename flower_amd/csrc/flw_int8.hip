@@ -190,7 +190,7 @@ __device__ __forceinline__ void int8_epilogue(const Int8Params& p, const v16i (&
 }
 
 // Any sizes and alignments: tiles of 64 (n) x 64 (m), 2 x 2 waves, 128 K bytes a stage through registers, three stages of them
-// under way, into two LDS buffers ([517, 1283] at K = 1291: ANYUS us; 22 with one stage under way). Behind K a load takes the row's
+// under way, into two LDS buffers ([517, 1283] at K = 1291: 11.5 us; 22 with one stage under way). Behind K a load takes the row's
 // last 16 bytes, and what it should not have is dropped on the way to LDS: no load stands in a branch. SHORT: K < 16.
 constexpr int kAnyAhead = 3;
 
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(64 * WN * WM) void int8_tile_kernel(Int8Params p) {
 template <int WN, int WM, int TN, int TM, bool TAIL, bool STREAM>
 __global__ __launch_bounds__(64 * WN * WM) void int8_stream_kernel(Int8Params p) {
   constexpr int BK = 128, BN = 32 * WN * TN, BM = 32 * WM * TM, NW = WN * WM, kStage = (BN + BM) * BK;
-  constexpr int RPI = 8, IPW = (BN + BM) / RPI / NW, CPK = 8;                    // rows a load, loads a wave and stage, chunks a row
+  constexpr int RPI = 8, IPW = (BN + BM) / RPI / NW;                             // rows a load, loads a wave and stage
   static_assert((BN + BM) % (RPI * NW) == 0 && BN % (RPI * IPW) == 0 && TN % 2 == 0, "a wave's loads are of one operand");
   __shared__ __align__(16) uint8_t lds[2 * kStage + NW * 4096];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -89,10 +89,33 @@ __device__ __forceinline__ void rows8_store(T* row, int c, int cols, const float
   }
 }
 
-// x / (1 + exp(-x)), the quotient by a reciprocal and one correction (the denominator within what fp32 can invert: x / d is 0 there).
+// x / (1 + exp(-x)): the exponent -x / ln 2 as a rounded product and what the rounding and the constant leave, which the power
+// takes as a factor 1 + ln 2 * rest; the quotient by a reciprocal and one correction. x from 87 on, and 0 (|silu| < 2e-36) below
+// -87, infinities included: between, fp32 holds the power and its inverse. [65536, 4096]: 228 us into int8 (5.9 TB/s), 256 with expf.
 __device__ __forceinline__ float silu(float x) {
-  const float d = fminf(1.0f + expf(-x), 1e38f), r = __builtin_amdgcn_rcpf(d), q = x * r;
-  return fmaf(fmaf(-q, d, x), r, q);
+  constexpr float L = 1.44269502162933350f, REST = 1.92596298e-8f, LN2 = 0.69314718f;            // 1 / ln 2 = L + REST
+  const float hi = -x * L, lo = fmaf(-x, REST, fmaf(-x, L, -hi)), e = __builtin_amdgcn_exp2f(hi);
+  const float d = 1.0f + fmaf(e, lo * LN2, e), r = __builtin_amdgcn_rcpf(d), q = x * r, v = fmaf(fmaf(-q, d, x), r, q);
+  return x > 87.0f ? x : x < -87.0f ? 0.0f : v;
+}
+
+// x Phi(x) = max(x, 0) - |x| Q(|x|), where Q(z) = 1 - Phi(z) = exp(-z^2 / 2) R(z). R is smooth and slow, as 1 / z is: a polynomial of
+// degree 8 in t = 1 / (1 + 0.295 z), fitted to z <= 14 (relative error 3.7e-8; Q(14) is below fp32). One exponential, one
+// reciprocal and 8 products, where erff takes a wave of mixed values through both of its ranges, and no loss at negative x, where
+// 1 + erf cancels: within 2e-7 |x| everywhere, 3.3e-8 of the size over normal x (erff's form: 3.8e-8). -inf gives the limit, 0.
+// [32768, 4096] into e4m3: 110 us, 129 with erff.
+__device__ __forceinline__ float gelu(float x) {
+  const float z = fminf(fabsf(x), 16.0f), t = __builtin_amdgcn_rcpf(fmaf(0.295f, z, 1.0f));
+  float r = 0.03942114859819412f;
+  r = fmaf(r, t, -0.18340615928173065f);
+  r = fmaf(r, t, 0.27101656794548035f);
+  r = fmaf(r, t, -0.11707105487585068f);
+  r = fmaf(r, t, 0.16628894209861755f);
+  r = fmaf(r, t, 0.08474481850862503f);
+  r = fmaf(r, t, 0.12169938534498215f);
+  r = fmaf(r, t, 0.11728934198617935f);
+  r = fmaf(r, t, 1.7006914276862517e-05f);
+  return fmaf(-z * __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f), r, x < 0.0f ? 0.0f : x);
 }
 
 // One value of every lane of a row, combined over the row's LPR lanes (the same bits in all of them).
@@ -176,7 +199,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] = 0.5f * f[i][e] * (1.0f + erff(f[i][e] * 0.70710678118654752f));
+      for (int e = 0; e < 8; ++e) f[i][e] = gelu(f[i][e]);
   }
   uint32_t m = 0;                                  // |h| as bit patterns: NaN above infinity above the rest
 #pragma unroll

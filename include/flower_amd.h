@@ -631,7 +631,7 @@ int flw_fp8_scaled_mm_residual(const uint8_t* x8, int64_t M, int64_t K, const ui
  *   flw_rows8_rmsnorm  h = t / sqrt(mean(t^2) + eps) * weight[cols], t = x, or with a residual t = x + residual rounded to x's
  *                      type and written to sum (the sum may not overlap an input);
  *   flw_rows8_gelu     h = 0.5 x (1 + erf(x / sqrt 2));
- *   flw_rows8_swiglu   h = gate / (1 + exp(-gate)) * up.
+ *   flw_rows8_swiglu   h = gate / (1 + exp(-gate)) * up;  both activations have their limits at infinity, 0 at -inf.
  * dtype: fp32 or bf16, of x, residual, sum, gate and up; weight fp32 or of that type. Row strides in elements, at least cols,
  * any alignment (16-byte rows are read faster). cols <= 32768. codes: bytes, row stride at least cols; the bytes behind a row
  * stay as they are. */

@@ -7,6 +7,8 @@ for erf, exp, the sum and the quotient, 2^-21 of |x| (|h| for SwiGLU) with a mar
 A bf16 result is at most 2^-8 from its value (half a step of the coarsest place), each further rounding 2^-8 of what it rounds.
 """
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -14,6 +16,7 @@ import torch
 from flower_amd.kernels import gelu_quant, int8_linear, int8_scaled_mm, quant_rows, rms_norm_quant, swiglu_quant
 from oracle import int8 as O
 from oracle.e4m3 import e4m3_to_f32
+from oracle.int8 import gelu
 from tests.gpu_util import seeded, to_np
 
 pytestmark = pytest.mark.gpu
@@ -105,6 +108,38 @@ def test_rows_that_are_not_finite_or_tiny(cols):
         assert torch.isnan(scale[0]) and not codes[0].any() and torch.isfinite(scale[[3, 5, 6]]).all()
     y = int8_linear(x[[0, 5, 1, 6]], torch.ones(3, cols, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"))
     assert torch.isnan(y[[0, 2]]).all() and torch.isfinite(y[[1, 3]]).all()
+
+
+def test_infinities_into_e4m3():
+    """What an activation makes of an infinity is its limit: inf at inf and 0 at -inf. A row that holds an infinity has an infinite
+    scale, and with it codes 0 but for its own."""
+    x = torch.ones(4, 64, device="cuda")
+    x[0, 3], x[1, 4], x[2, 5] = float("inf"), -float("inf"), float("nan")
+    codes, scale = gelu_quant(x, dtype=torch.float8_e4m3fn)
+    assert torch.isinf(scale[0]) and torch.isnan(scale[2]) and torch.isfinite(scale[[1, 3]]).all()
+    assert torch.isnan(codes[0, 3].float()) and codes[0, 4].float() == 0 and codes[1, 4].float() == 0
+    want = 0.5 * (1 + math.erf(math.sqrt(0.5)))
+    assert (codes[1, 0].float() * scale[1] - want).abs() <= want * 2 ** -4 and torch.equal(codes[1, 5:], codes[3, 5:])
+    codes, scale = swiglu_quant(x, torch.ones_like(x), dtype=torch.float8_e4m3fn)
+    assert torch.isinf(scale[0]) and torch.isnan(scale[2]) and torch.isfinite(scale[[1, 3]]).all() and codes[1, 4].float() == 0
+    for quant in (gelu_quant, lambda t: swiglu_quant(t, torch.ones_like(t))):       # the largest that are finite stay so
+        big = torch.full((1, 64), 3e38, device="cuda")
+        codes, scale = quant(big)
+        assert torch.isfinite(scale).all() and (codes == 127).all()
+        codes, scale = quant(-big)
+        assert torch.isfinite(scale).all() and not codes.any()
+
+
+def test_gelu_of_far_values():
+    """Rows of negative values alone, where gelu is small: 2^-19 relative down to -6 (the exponential's argument z^2 / 2 = 18 is off
+    by its own 2^-24 three times: its constant, z^2 and the product, 18 * 3 * 2^-24 = 2^-18.2 at most), and the codes' half step."""
+    for lo, hi in ((-1.0, -0.1), (-3.0, -2.0), (-6.0, -5.0)):
+        x = torch.linspace(lo, hi, 512, device="cuda").reshape(4, 128)
+        codes, scale = gelu_quant(x)
+        h = torch.from_numpy(gelu(to_np(x)))
+        got = codes.cpu().double() * scale.cpu().double()[:, None]
+        peak = h.abs().amax(1, keepdim=True)
+        assert ((got - h).abs() <= peak * (0.5 / 127 + 2.0 ** -17)).all()
 
 
 def test_rows_of_any_stride_and_shape():
