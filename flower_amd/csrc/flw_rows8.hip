@@ -249,19 +249,21 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows8_kernel(Rows8Param
 }
 
 // Column sums of bf16 rows (a bias's gradient), in two passes of a fixed order: each workgroup sums 512 columns (8 a lane) of
-// kSumRows rows, its four waves every fourth row, into part [chunks][cols]; then the chunks of each column are summed.
-constexpr int kSumRows = 128;
+// a chunk of rows, its four waves every fourth row, into part [chunks][cols]; then the chunks of each column are summed. Chunks of
+// 128 rows, of 32 for few rows, which 128 would leave to a few workgroups (both launches, us, at 32 / 128: [64, 1280] 4.5 / 4.9,
+// [517, 1280] 4.8 / 5.9, [2048, 3840] 6.3 / 6.6, [4096, 5120] 12.6 / 10.2; [16384, 5120] 28.8, 5.8 TB/s).
+constexpr int64_t sum_rows(int64_t rows) { return rows <= 2048 ? 32 : 128; }
 
 template <bool ALIGNED>
 __global__ __launch_bounds__(256) void col_sum_kernel(const uint16_t* __restrict__ x, int64_t rows, int cols, int64_t xs,
-                                                      float* __restrict__ part) {
+                                                      int chunk, float* __restrict__ part) {
   __shared__ float fold[3][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 512 + 8 * lane;
-  const int64_t r1 = min(rows, (int64_t)(blockIdx.y + 1) * kSumRows);
+  const int64_t r1 = min(rows, (int64_t)(blockIdx.y + 1) * chunk);
   float acc[8] = {};
   if (c < cols) {
 #pragma unroll 4
-    for (int64_t r = (int64_t)blockIdx.y * kSumRows + wave; r < r1; r += 4) {
+    for (int64_t r = (int64_t)blockIdx.y * chunk + wave; r < r1; r += 4) {
       float f[8];
       rows8_load<uint16_t, ALIGNED>(x + r * xs, c, cols, f);
 #pragma unroll
@@ -392,7 +394,7 @@ extern "C" int flw_rows8_swiglu(const void* gate, const void* up, int dtype, int
   return rows8<kRows8Swiglu>(p, dtype, cols, dtype, code_type, stream, "flw_rows8_swiglu");
 }
 
-static int64_t sum_chunks(int64_t rows) { return (rows + kSumRows - 1) / kSumRows; }
+static int64_t sum_chunks(int64_t rows) { return (rows + sum_rows(rows) - 1) / sum_rows(rows); }
 
 extern "C" size_t flw_col_sum_workspace_bytes(int64_t rows, int64_t cols) {
   return rows <= 0 || cols <= 0 ? 0 : (size_t)(sum_chunks(rows) * cols * 4);
@@ -415,7 +417,7 @@ extern "C" int flw_col_sum(const void* x, int64_t rows, int64_t cols, int64_t x_
   float* part = static_cast<float*>(workspace);
   (void)launch_args(aligned ? reinterpret_cast<const void*>(&col_sum_kernel<true>) : reinterpret_cast<const void*>(&col_sum_kernel<false>),
                     dim3((unsigned)((cols + 511) / 512), (unsigned)chunks), dim3(256), 0, s, tm.start, nullptr,
-                    static_cast<const uint16_t*>(x), rows, (int)cols, x_row_stride, part);
+                    static_cast<const uint16_t*>(x), rows, (int)cols, x_row_stride, (int)sum_rows(rows), part);
   (void)launch_args(reinterpret_cast<const void*>(&col_sum_fold_kernel), dim3((unsigned)((cols + 15) / 16)), dim3(256), 0, s, nullptr,
                     tm.stop, static_cast<const float*>(part), chunks, (int)cols, out, (int)(out_dtype == FLW_F32));
   return check_launch("flw_col_sum");

@@ -11,7 +11,7 @@ import pytest
 import torch
 import torch.nn as nn
 
-from flower_amd import int8
+from flower_amd import _lib, int8
 from flower_amd.kernels import int8_linear, quant_rows
 from flower_amd.precision import fp8_weight_cache
 from oracle.gemm import fp8_linear_backward
@@ -87,6 +87,24 @@ def test_bf16_backward_of_odd_widths_and_on_request(N, K):
         plain = [t.detach().requires_grad_() for t in (x, w, b)]
         got = torch.autograd.grad(int8.int8_linear_train(*plain), plain, g)
         assert torch.equal(got[0], x.grad) and torch.equal(got[1], mod.weight.grad) and torch.equal(got[2], mod.bias.grad)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 32, 33, 2048, 2049, 5000])
+@pytest.mark.parametrize("cols,stride", [(1, 1), (7, 7), (8, 24), (513, 520), (1280, 1280)])
+def test_column_sums(rows, cols, stride):
+    """Chains of at most 32 + 3 + 3 + 16 additions in fp32 of any rows here, each off by 2^-24 of the absolute sum; then the type's
+    rounding. The same bits every time."""
+    lib = _lib.load()
+    x = seeded((rows, stride), 8, torch.bfloat16)[:, :cols]
+    want, total = x.double().sum(0), x.double().abs().sum(0)
+    ws = torch.empty(lib.flw_col_sum_workspace_bytes(rows, cols), dtype=torch.uint8, device="cuda")
+    for dtype, code, half in ((torch.float32, _lib.F32, 0.0), (torch.bfloat16, _lib.BF16, 2.0 ** -8)):
+        out = torch.full((2, cols + 1), 7.0, dtype=dtype, device="cuda")
+        for o in out:
+            ws.fill_(255)
+            _lib.check(lib.flw_col_sum(x.data_ptr(), rows, cols, stride, o.data_ptr(), code, ws.data_ptr(), ws.numel(), _lib.stream_of(x)), "sum")
+        assert torch.equal(out[0], out[1]) and (out[:, cols] == 7).all()
+        assert ((out[0, :cols].double() - want).abs() <= want.abs() * half + total * 54 * 2.0 ** -24 * (1 + half)).all()
 
 
 def test_empty_batch():

@@ -133,3 +133,14 @@ def test_c_entries_refuse_on_the_host():
                                                    ys=8, ws=P, wb=need, stream=None), **k}.values())
     for change, rc in ((dict(wb=need - 1), 3), (dict(ws=None), 3), (dict(ws=P + 8), 3), (dict(K=0), 1), (dict(M=-1), 1)):
         assert lin(**change) == rc, change
+    act = lambda **k: lib.flw_rows8_swiglu(*{**dict(x=P, u=P, dtype=1, rows=2, cols=64, xs=64, us=64, type=2, codes=P, cs=64, scale=P, stream=None),  # noqa: E731
+                                             **k}.values())
+    for change, rc in ((dict(u=None), 1), (dict(us=63), 1), (dict(u=P + 1), 1), (dict(dtype=2), 2), (dict(type=0), 2)):
+        assert act(**change) == rc, change
+    assert lib.flw_rows8_gelu(P, 1, 2, 64, 63, 3, P, 64, P, None) == 1
+    # chunks of 32 rows, of 128 from 2049 rows on
+    assert [lib.flw_col_sum_workspace_bytes(r, 5) for r in (0, 1, 33, 2048, 2049)] == [0, 20, 40, 1280, 340]
+    tot = lambda **k: lib.flw_col_sum(*{**dict(x=P, rows=3, cols=5, xs=5, out=P, dtype=0, ws=P, wb=20, stream=None), **k}.values())  # noqa: E731
+    for change, rc in ((dict(x=None), 1), (dict(out=None), 1), (dict(rows=0), 1), (dict(cols=0), 1), (dict(xs=4), 1), (dict(dtype=3), 2), (dict(wb=19), 3),
+                       (dict(ws=None), 3), (dict(ws=P + 4), 3), (dict(x=P + 1), 1), (dict(out=P + 2), 1), (dict(rows=2 ** 24, wb=2 ** 30), 2)):
+        assert tot(**change) == rc, change
