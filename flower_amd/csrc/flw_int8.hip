@@ -783,7 +783,8 @@ static int int8_mm(Int8Params p, int64_t M, int64_t N, int64_t K, int64_t sa_cou
   const Int8Kernel k = vector ? kernel_of(p) : Int8Kernel{K < 16 ? reinterpret_cast<const void*>(&int8_any_kernel<true>) : reinterpret_cast<const void*>(&int8_any_kernel<false>),
                                                        64, 64, 256, false};
   const int64_t tiles_n = (N + k.bn - 1) / k.bn, tiles_m = (M + k.bm - 1) / k.bm;
-  FLW_REQUIRE(tiles_n * tiles_m <= 0x3FFFFFFFll, FLW_E_UNSUPPORTED, "too many output tiles");
+  FLW_REQUIRE(k.persistent ? tiles_n * tiles_m <= 0x3FFFFFFFll : tiles_n * tiles_m * k.threads <= 0xFFFFFFFFll, FLW_E_UNSUPPORTED,
+              "too many output tiles");         // a launch holds fewer than 2^32 threads
   p.tiles_n = (int)tiles_n;
   p.tiles_m = (int)tiles_m;
   const int64_t grid = k.persistent ? std::min<int64_t>(tiles_n * tiles_m, compute_units()) : tiles_n * tiles_m;

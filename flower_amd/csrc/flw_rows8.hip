@@ -349,9 +349,9 @@ static int rows8(Rows8Params p, int dtype, int64_t cols, int weight_dtype, int c
   const int nc = (int)((cols + 8 * lpr - 1) / (8 * lpr));
   const void* kernel = dtype == FLW_F32 ? (aligned ? rows8_of<float, OP, true>(lpr, nc) : rows8_of<float, OP, false>(lpr, nc))
                                         : (aligned ? rows8_of<uint16_t, OP, true>(lpr, nc) : rows8_of<uint16_t, OP, false>(lpr, nc));
-  const int64_t rpb = lpr == 64 ? 4 : 1;
-  (void)launch_timed(kernel, dim3((unsigned)((p.rows + rpb - 1) / rpb)), dim3((unsigned)(lpr == 64 ? 256 : lpr)),
-                     static_cast<hipStream_t>(stream), p);
+  const int64_t rpb = lpr == 64 ? 4 : 1, groups = (p.rows + rpb - 1) / rpb, threads = lpr == 64 ? 256 : lpr;
+  FLW_REQUIRE(groups * threads <= 0xFFFFFFFFll, FLW_E_UNSUPPORTED, "too many rows");       // a launch holds fewer than 2^32 threads
+  (void)launch_timed(kernel, dim3((unsigned)groups), dim3((unsigned)threads), static_cast<hipStream_t>(stream), p);
   return check_launch(name);
 }
 

@@ -305,3 +305,31 @@ def test_on_a_stream_of_its_own_and_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(held, step()))
+
+
+def test_offsets_past_32_bits():
+    """Rows more than 2^32 bytes apart, and an output of more than that: each as at its place in a small one."""
+    K, N, far = 144, 40, 2 ** 31 + 64
+    base = torch.empty(2 * far + K, dtype=torch.bfloat16, device="cuda")
+    x = base.as_strided((3, K), (far, 1))
+    x.copy_(seeded((3, K), 1, torch.bfloat16))
+    near = x.contiguous()
+    for got, want in zip((*quant_rows(x), *swiglu_quant(x, x), *rms_norm_quant(x, near[0], residual=x)),
+                         (*quant_rows(near), *swiglu_quant(near, near), *rms_norm_quant(near, near[0], residual=near))):
+        assert torch.equal(got, want)
+    w8, sw = quant_rows(seeded((N, K), 2, torch.bfloat16))
+    assert torch.equal(int8_linear(x, w8, sw), int8_linear(near, w8, sw))
+    bytes_ = base.view(torch.int8).as_strided((3, K), (2 * far, 1))
+    codes, s = quant_rows(near)
+    bytes_.copy_(codes)
+    assert torch.equal(int8_scaled_mm(bytes_, s, w8, sw), int8_scaled_mm(codes, s, w8, sw))
+    assert torch.equal(int8_scaled_mm(w8, sw, bytes_, s), int8_scaled_mm(w8, sw, codes, s))
+    del base, x, bytes_
+    for M, N, K in ((70000, 32768, 144), (70000, 32768, 128), (70001, 32767, 40)):      # the stream, tiles, any
+        a, b = (torch.randint(-128, 128, (r, K), dtype=torch.int8, device="cuda") for r in (M, N))
+        sa, sb = torch.rand(M, device="cuda"), torch.rand(N, device="cuda")
+        y = int8_scaled_mm(a, sa, b, sb)
+        assert y.numel() * 2 > 2 ** 32
+        for rows in (slice(0, 40), slice(M // 2, M // 2 + 33), slice(M - 50, M)):
+            assert torch.equal(y[rows], int8_scaled_mm(a[rows], sa[rows], b, sb))
+        del y

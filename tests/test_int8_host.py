@@ -115,6 +115,8 @@ def test_c_entries_refuse_on_the_host():
                        (dict(x=P + 1), 1)):
         assert rows(**change) == rc, change
     assert rows(rows=0, x=None) == 0
+    for cols, most in ((512, 2 ** 26), (2048, 2 ** 26), (8192, 2 ** 24), (8200, 2 ** 22)):        # a launch's 2^32 threads
+        assert rows(rows=most, cols=cols, xs=cols, cs=cols) == 2, cols
     norm = lambda **k: lib.flw_rows8_rmsnorm(*{**dict(x=P, a=P, dtype=1, rows=2, cols=64, xs=64, as_=64, w=P, wd=1, eps=0.0, sum=P, ss=64, type=3,  # noqa: E731
                                                       codes=P, cs=64, scale=P, stream=None), **k}.values())
     for change, rc in ((dict(sum=None), 1), (dict(w=None), 1), (dict(wd=2), 2), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1), (dict(as_=8), 1), (dict(ss=8), 1),
@@ -127,6 +129,7 @@ def test_c_entries_refuse_on_the_host():
                        (dict(y=P + 1), 1), (dict(M=-1), 1), (dict(N=2 ** 31), 2)):
         assert mm(**change) == rc, change
     assert mm(M=0, a=None, sac=0) == 0
+    assert mm(M=2 ** 30, sac=1, N=64, sbc=1, ys=64, K=65, as_=65, bs=65) == 2 and b"tiles" in lib.flw_last_error()
     need = lib.flw_int8_linear_workspace_bytes(3, 65)
     assert need == 3 * 80 + 12
     lin = lambda **k: lib.flw_int8_linear(*{**dict(x=P, dtype=1, M=3, K=65, xs=65, b=P, N=8, bs=65, sb=P, sbc=8, bias=None, bd=1, res=None, rs=0, y=P,  # noqa: E731
