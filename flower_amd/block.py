@@ -38,6 +38,7 @@ from . import _lib
 from .attention import CausalSelfAttention
 from .kernels.fp8_swa_attention import (fp8_swa_attention_forward, fp8_swa_attention_from_codes,
                                         qk_norm_rope_quant_e4m3)
+from .int8 import Int8Linear
 from .kernels.int8 import gelu_quant, rms_norm_quant, swiglu_quant
 from .precision import Fp8Linear
 
@@ -501,11 +502,11 @@ class TransformerBlock(nn.Module):
         self.ff = FeedForward(config)
 
     def _int8_ok(self, x: torch.Tensor) -> bool:
-        from .int8 import Int8Linear
-        return (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 3 and x.numel() > 0 and not torch.is_grad_enabled()
+        return (type(self.attn.qkv) is Int8Linear and not torch.is_grad_enabled()
+                and x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 3 and x.numel() > 0
                 and not torch.is_autocast_enabled("cuda") and x.shape[-1] <= 32768 and self.ff.linears()[-1].in_features <= 32768
                 and all(w.dtype in (torch.bfloat16, torch.float32) for w in (self.ln1.weight, self.ln2.weight))
-                and all(type(m) is Int8Linear for m in (self.attn.qkv, self.attn.out, *self.ff.linears())))
+                and all(type(m) is Int8Linear for m in (self.attn.out, *self.ff.linears())))
 
     def _forward_int8(self, x: torch.Tensor, attend) -> torch.Tensor:
         """The block with int8 linears; attend: from the qkv projection to what ``out`` takes. The norms' outputs stay in fp32 up to

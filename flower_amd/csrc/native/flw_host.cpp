@@ -763,6 +763,18 @@ Tensor as_rows(const Tensor& x, int64_t* ld) {
   return y;
 }
 
+// As as_rows, for the casts that take 16-byte rows: a stride of whole 8 values and an aligned start, or a copy.
+Tensor vector_rows(const Tensor& x) {
+  int64_t ld;
+  Tensor y = as_rows(x, &ld);
+  const int64_t K = y.size(1);
+  if (ld % 8 != 0 || reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 != 0) {
+    y = y.clone(at::MemoryFormat::Contiguous);
+    ld = K;
+  }
+  return y.stride(0) == ld ? y : y.as_strided({y.size(0), K}, {ld, 1});     // one row, of any stride
+}
+
 at::ScalarType code_dtype(bool e4m3) { return e4m3 ? at::kFloat8_e4m3fn : at::kChar; }
 
 void check_float_rows(const char* what, const Tensor& x) {
@@ -943,27 +955,30 @@ std::tuple<OptTensor, OptTensor, OptTensor> int8_linear_bwd(const Tensor& g0, co
                                                             bool need_w, const std::optional<at::ScalarType>& bias_dtype, int64_t stream) {
   c10::DeviceGuard guard(x0.device());
   const int64_t N = weight.size(0), K = weight.size(1);
-  const Tensor g = rows16(g0.reshape({-1, N}).to(at::kBFloat16));
+  int64_t gs;
+  Tensor g = as_rows(g0.to(at::kBFloat16), &gs);
+  if (need_x || need_w) {
+    g = vector_rows(g);
+    gs = g.stride(0);
+  }
   const int64_t M = g.size(0), ld = (M + 127) / 128 * 128;
   OptTensor dx, dw, db;
   if (need_x) {
     Rows8 rows(g, true);
-    check(flw_rows8(g.data_ptr(), FLW_BF16, M, N, M > 1 ? g.stride(0) : N, FLW_E4M3, rows.codes.data_ptr(), N, f32(rows.scale),
-                    str(stream)),
+    check(flw_rows8(g.data_ptr(), FLW_BF16, M, N, gs, FLW_E4M3, rows.codes.data_ptr(), N, f32(rows.scale), str(stream)),
           "int8 linear backward");
-    const auto cols = w_cols ? std::make_tuple(w_cols->first, w_cols->second) : quant_cols(rows16(weight), true, N, stream);
+    const auto cols = w_cols ? std::make_tuple(w_cols->first, w_cols->second) : quant_cols(vector_rows(weight), true, N, stream);
     dx = scaled_mm(rows.codes, rows.scale, std::get<0>(cols), std::get<1>(cols), std::nullopt, true, stream);
   }
   if (need_w) {
-    const auto [g8, gs] = quant_cols(g, true, ld, stream);
-    const auto [x8, xs] = quant_cols(rows16(x0.reshape({-1, K})), true, ld, stream);
-    dw = scaled_mm(g8, gs, x8, xs, std::nullopt, true, stream);
+    const auto [g8, g_scale] = quant_cols(g, true, ld, stream);
+    const auto [x8, x_scale] = quant_cols(vector_rows(x0), true, ld, stream);
+    dw = scaled_mm(g8, g_scale, x8, x_scale, std::nullopt, true, stream);
   }
   if (bias_dtype) {
     db = empty(g, {N}, *bias_dtype == at::kFloat ? at::kFloat : at::kBFloat16);
     const Tensor ws = workspace(g, flw_col_sum_workspace_bytes(M, N));
-    check(flw_col_sum(g.data_ptr(), M, N, M > 1 ? g.stride(0) : N, db->data_ptr(), dtype_code(*db), ws.data_ptr(), (size_t)ws.numel(),
-                      str(stream)),
+    check(flw_col_sum(g.data_ptr(), M, N, gs, db->data_ptr(), dtype_code(*db), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
           "int8 linear backward");
   }
   return {dx, dw, db};

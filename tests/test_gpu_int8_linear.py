@@ -89,6 +89,36 @@ def test_bf16_backward_of_odd_widths_and_on_request(N, K):
         assert torch.equal(got[0], x.grad) and torch.equal(got[1], mod.weight.grad) and torch.equal(got[2], mod.bias.grad)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 48, 64), (70, 48, 64), (70, 33, 40)])
+def test_gradients_of_any_layout(M, N, K):
+    """Inputs and an output's gradient that do not start on 16 bytes, with odd or no strides, or all one row: as their copies."""
+    x, w, b, g = tensors(M, N, K)
+
+    def grads(x, w, g):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = int8.int8_linear_train(*leaves)
+        return (y.detach(), *torch.autograd.grad(y, leaves, g))
+
+    def odd(t):
+        out = torch.empty(t.shape[0], t.shape[1] + 3, dtype=t.dtype, device="cuda")[:, :t.shape[1]]
+        return out.copy_(t)
+
+    def shifted(t):
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+
+    def columns(t):
+        return t.t().contiguous().t()
+
+    one = seeded((N,), 9, torch.bfloat16)
+    for a, v, h in ((odd(x), w, g), (shifted(x), shifted(w), shifted(g)), (x, odd(w), odd(g)), (columns(x), columns(w), columns(g)),
+                    (x, w, one.expand(M, N)), (x, w, one[:1].expand(M, N)), (x[:1].expand(M, K), w, g)):
+        for got, want in zip(grads(a, v, h), grads(a.contiguous().clone(), v.contiguous().clone(), h.contiguous().clone())):
+            assert torch.equal(got, want)
+    leaf = x.clone().requires_grad_()
+    int8.int8_linear_train(leaf, w).sum(0).pow(2).sum().backward()                      # a gradient that autograd expands
+    assert leaf.grad.any()
+
+
 @pytest.mark.parametrize("rows", [1, 3, 32, 33, 2048, 2049, 5000])
 @pytest.mark.parametrize("cols,stride", [(1, 1), (7, 7), (8, 24), (513, 520), (1280, 1280)])
 def test_column_sums(rows, cols, stride):
