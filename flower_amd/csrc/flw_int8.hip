@@ -39,7 +39,7 @@ struct Int8Params {
   int x32;
   int M, N, K;
   int tiles_n, tiles_m;
-  int wide;                // N % 8 == 0, rows of y and of the residual start on 16 bytes, sb too, one a column
+  int wide;                // N % 8 == 0, rows of y and of the residual start on 16 bytes, fewer than 2^26 apart, sb too, one a column
 };
 
 // 16 bytes at any address.
@@ -129,15 +129,20 @@ __device__ __forceinline__ uint4 int8_plus(uint4 x, uint4 y) {
   return make_uint4(bf16x2_rne(a[0], a[1]), bf16x2_rne(a[2], a[3]), bf16x2_rne(a[4], a[5]), bf16x2_rne(a[6], a[7]));
 }
 
+// 8 bf16 values to an aligned place; STREAM: past the caches.
+template <bool STREAM>
+__device__ __forceinline__ void int8_put(uint16_t* y, uint4 o) {
+  if (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(v4i, o), reinterpret_cast<v4i*>(y));
+  else *reinterpret_cast<uint4*>(y) = o;
+}
+
 // The 8 bf16 values o of row m from column n on (n % 8 == 0, m < M, n < N) into y, the residual added.
-template <bool WIDE = false, bool STREAM = false>
 __device__ __forceinline__ void int8_store8(const Int8Params& p, int m, int n, uint4 o) {
   uint16_t* y = p.y + (int64_t)m * p.ys + n;
   const uint16_t* res = p.res ? p.res + (int64_t)m * p.rs + n : nullptr;
-  if (WIDE || p.wide) {
+  if (p.wide) {
     if (res) o = int8_plus(o, *reinterpret_cast<const uint4*>(res));
-    if (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(v4i, o), reinterpret_cast<v4i*>(y));
-    else *reinterpret_cast<uint4*>(y) = o;
+    int8_put<false>(y, o);
     return;
   }
   float a[8];
@@ -372,7 +377,7 @@ __global__ __launch_bounds__(64 * WN * WM) void int8_tile_kernel(Int8Params p) {
 // Two sets of fragments, a quarter of a stage (32 of K) each: while a quarter's products run, the next one's fragments are read,
 // across the stage's barrier and the tile's end too. The order of a quarter is kept as it is written: a product, then part of the
 // reads and loads, so that the wave issues none of them in a burst.
-template <int WN, int WM, int TN, int TM, bool TAIL, bool STREAM>
+template <int WN, int WM, int TN, int TM, bool TAIL, bool STREAM, bool RES>
 __global__ __launch_bounds__(64 * WN * WM) void int8_stream_kernel(Int8Params p) {
   constexpr int BK = 128, BN = 32 * WN * TN, BM = 32 * WM * TM, NW = WN * WM, kStage = (BN + BM) * BK;
   constexpr int RPI = 8, IPW = (BN + BM) / RPI / NW;                             // rows a load, loads a wave and stage
@@ -458,41 +463,80 @@ __global__ __launch_bounds__(64 * WN * WM) void int8_stream_kernel(Int8Params p)
   using X2 = std::integral_constant<int, 2>;
   using X3 = std::integral_constant<int, 3>;
 
-  // The tile at m0, n0: each wave 32 x 32 values at a time through its own LDS (2 KB, in turn two of them; row r: 64 bytes, 16-byte
-  // chunk c at c ^ (r / 4 % 4)).
+  // The tile at m0, n0: each wave 32 columns of its rows at a time through its own LDS (2 KB for 32 x 32 of them; row r: 64 bytes,
+  // 16-byte chunk c at c ^ (r / 4 % 4)). A lane holds the scales and biases of columns 64 k + lane and hands them to the others; the
+  // residual's next columns are under way while these are written ([16384, 5120] at K = 1280 with a residual 162 us, 180 with each
+  // load where it is used; with a bias 117 and 133). Rows are reached by 32-bit offsets (checked on the host).
+  static_assert(TM * 2048 <= 4096 && TN % 2 == 0, "the wave's own LDS");
   uint8_t* const own = lds + 2 * kStage + wave * 4096;
   auto write_out = [&](int m0, int n0) __attribute__((always_inline)) {
-    const int mw = m0 + 32 * TM * wm, nw = n0 + 32 * TN * wn;
-    float sa[TM];
-#pragma unroll
-    for (int j = 0; j < TM; ++j) sa[j] = p.sa[(int64_t)min(mw + 32 * j + (lane & 31), p.M - 1) * p.sa_step];
-    each_up<TN>([&](auto ic) __attribute__((always_inline)) {
+    int ln = lane;                                // the places below are worked out here, not held in registers through the stages
+    asm volatile("" : "+v"(ln));
+    const int h = ln >> 5, mw = min(m0 + 32 * TM * wm, p.M - 1), nw = min(n0 + 32 * TN * wn, p.N - 8);      // a wave without rows or columns: the last ones
+    const bool some = m0 + 32 * TM * wm < p.M && n0 + 32 * TN * wn < p.N;
+    const uint16_t* const res_w = RES ? p.res + (int64_t)mw * p.rs + nw : nullptr;
+    uint16_t* const y_w = p.y + (int64_t)mw * p.ys + nw;
+    const uint32_t rs = RES ? (uint32_t)p.rs : 0, ys = (uint32_t)p.ys;
+    uint4 res[2][TM][2];
+    auto fetch = [&](auto ic) __attribute__((always_inline)) {
       constexpr int i = decltype(ic)::value;
-      float sb[16], bias[16];
-      int8_columns(p, nw + 32 * i + 4 * hh, sb, bias);
-      each_up<TM>([&](auto jc) __attribute__((always_inline)) {
-        constexpr int j = decltype(jc)::value;
-        uint8_t* piece = own + (i * TM + j & 1) * 2048;
+      const uint32_t n = min(32 * i + 8 * (ln & 3), p.N - 8 - nw);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = int8_value(acc[i][j][4 * g + e], sa[j], sb[4 * g + e], bias[4 * g + e]);
-          *reinterpret_cast<uint2*>(piece + (lane & 31) * 64 + 16 * (g ^ ((lane >> 2) & 3)) + 8 * hh) =
-              make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
-        }
-        acc[i][j] = v16i{};
-        __builtin_amdgcn_s_waitcnt(0xC07F);       // lgkmcnt(0): the wave's own writes
-        asm volatile("" ::: "memory");
-        const int n = nw + 32 * i + 8 * (lane & 3);
+      for (int j = 0; j < TM; ++j)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const int r = 16 * q + (lane >> 2), m = mw + 32 * j + r;
-          const uint4 o = *reinterpret_cast<const uint4*>(piece + r * 64 + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
-          if (m < p.M && n < p.N) int8_store8<true, STREAM>(p, m, n, o);
+          const uint32_t m = min(32 * j + 16 * q + (ln >> 2), p.M - 1 - mw);
+          res[i & 1][j][q] = *reinterpret_cast<const uint4*>(res_w + (m * rs + n));
         }
-        asm volatile("" ::: "memory");
-      });
+    };
+    float sa[TM], sbl[TN / 2], bl[TN / 2];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) sa[j] = p.sa[(int64_t)min(mw + 32 * j + (ln & 31), p.M - 1) * p.sa_step];
+#pragma unroll
+    for (int k = 0; k < TN / 2; ++k) {
+      const int n = min(nw + 64 * k + ln, p.N - 1);
+      sbl[k] = p.sb[n];
+      bl[k] = int8_bias(p, n);
+    }
+    if (RES) fetch(std::integral_constant<int, 0>{});
+    asm volatile("" ::: "memory");
+    each_up<TN>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (RES && i + 1 < TN) fetch(std::integral_constant<int, i + 1>{});
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float sb[4], bias[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int from = 16 * h + 4 * (32 * (i & 1) + 8 * g + e);               // bytes
+          sb[e] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(sbl[i / 2])));
+          bias[e] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(bl[i / 2])));
+        }
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = int8_value(acc[i][j][4 * g + e], sa[j], sb[e], bias[e]);
+          *reinterpret_cast<uint2*>(own + j * 2048 + (ln & 31) * 64 + 16 * (g ^ ((ln >> 2) & 3)) + 8 * h) =
+              make_uint2(bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3]));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[i][j] = v16i{};
+      __builtin_amdgcn_s_waitcnt(0xC07F);         // lgkmcnt(0): the wave's own writes
+      asm volatile("" ::: "memory");
+      const int n = 32 * i + 8 * (ln & 3);
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int r = 16 * q + (ln >> 2), m = 32 * j + r;
+          uint4 o = *reinterpret_cast<const uint4*>(own + j * 2048 + r * 64 + 16 * ((ln & 3) ^ ((r >> 2) & 3)));
+          if (RES) o = int8_plus(o, res[i & 1][j][q]);
+          if (some && m < p.M - mw && n < p.N - nw) int8_put<STREAM>(y_w + ((uint32_t)m * ys + (uint32_t)n), o);
+        }
+      asm volatile("" ::: "memory");
     });
   };
 
@@ -715,10 +759,10 @@ static Int8Kernel tile_of(bool tail) {
                : reinterpret_cast<const void*>(&int8_tile_kernel<WN, WM, TN, TM, NST, false>),
           32 * WN * TN, 32 * WM * TM, 64 * WN * WM, false};
 }
-template <bool TAIL>
+template <bool TAIL, bool RES>
 static Int8Kernel stream_of(bool non_temporal) {
-  return {non_temporal ? reinterpret_cast<const void*>(&int8_stream_kernel<2, 4, 4, 2, TAIL, true>)
-                       : reinterpret_cast<const void*>(&int8_stream_kernel<2, 4, 4, 2, TAIL, false>),
+  return {non_temporal ? reinterpret_cast<const void*>(&int8_stream_kernel<2, 4, 4, 2, TAIL, true, RES>)
+                       : reinterpret_cast<const void*>(&int8_stream_kernel<2, 4, 4, 2, TAIL, false, RES>),
           256, 256, 512, true};
 }
 
@@ -739,7 +783,8 @@ static Int8Kernel kernel_of(const Int8Params& p) {
   if (rounds(128, 128, cus) == 1) return tile_of<4, 2, 1, 2, 3>(tail);
   if (p.K > 128 && p.wide && (double)rounds(256, 256, cus) <= 0.6 * (double)rounds(128, 128, 2 * cus)) {
     const bool past = M * N * 2 >= 64ll << 20;
-    return tail ? stream_of<true>(past) : stream_of<false>(past);
+    if (p.res != nullptr) return tail ? stream_of<true, true>(past) : stream_of<false, true>(past);
+    return tail ? stream_of<true, false>(past) : stream_of<false, false>(past);
   }
   return tile_of<4, 2, 1, 2, 2>(tail);
 }
@@ -778,7 +823,7 @@ static int int8_mm(Int8Params p, int64_t M, int64_t N, int64_t K, int64_t sa_cou
                      (size_t)few_lds_bytes(M, K), s, p, tm.start, tm.stop);
     return check_launch(name);
   }
-  p.wide = N % 8 == 0 && p.sb_step == 1 && (uintptr_t)p.sb % 16 == 0 && on16(p.y, 2 * p.ys, M) &&
+  p.wide = N % 8 == 0 && p.sb_step == 1 && std::max(p.ys, p.rs) < 1 << 25 && (uintptr_t)p.sb % 16 == 0 && on16(p.y, 2 * p.ys, M) &&
            (p.res == nullptr || on16(p.res, 2 * p.rs, M));
   const Int8Kernel k = vector ? kernel_of(p) : Int8Kernel{K < 16 ? reinterpret_cast<const void*>(&int8_any_kernel<true>) : reinterpret_cast<const void*>(&int8_any_kernel<false>),
                                                        64, 64, 256, false};
