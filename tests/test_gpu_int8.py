@@ -214,6 +214,19 @@ def test_large_products(M, N, K):
     assert torch.equal(int8_scaled_mm(a, sa, b, sb, bias=bias)[few], int8_scaled_mm(a[few], sa[few], b, sb, bias=bias))
 
 
+@pytest.mark.parametrize("M,N,K", [(4100, 2312, 256), (4096, 4096, 1296), (9000, 4104, 144)])
+def test_large_products_with_everything(M, N, K):
+    """Bias and a residual of its own row stride, over every row: as in parts of 200 rows, which another kernel computes."""
+    a, sa, b, sb = product(M, N, K)
+    wide, odd = seeded((M, N + 24), 1, torch.bfloat16), seeded((M, N + 3), 1, torch.bfloat16)
+    for bias in (seeded((N,), 2), seeded((N,), 2, torch.bfloat16), None):
+        for res in (wide[:, 8:8 + N], odd[:, 1:1 + N], None):
+            y = int8_scaled_mm(a, sa, b, sb, bias=bias, residual=res)
+            parts = [int8_scaled_mm(a[r:r + 200], sa[r:r + 200], b, sb, bias=bias, residual=None if res is None else res[r:r + 200])
+                     for r in range(0, M, 200)]
+            assert torch.equal(y, torch.cat(parts))
+
+
 @pytest.mark.parametrize("M", [1, 40, 700])
 def test_product_at_the_ends_of_its_range(M):
     """The longest K that int32 holds, with every product the largest: 128 * 128 * 131071 and its negative."""
