@@ -131,8 +131,8 @@ def test_infinities_into_e4m3():
 
 
 def test_gelu_of_far_values():
-    """Rows of negative values alone, where gelu is small: 2^-19 relative down to -6 (the exponential's argument z^2 / 2 = 18 is off
-    by its own 2^-24 three times: its constant, z^2 and the product, 18 * 3 * 2^-24 = 2^-18.2 at most), and the codes' half step."""
+    """Rows of negative values alone, where gelu is small: the exponential's argument, z^2 / 2 = 18 at -6, is off by its own 2^-24
+    three times (its constant, z^2, the product), 18 * 3 * 2^-24 = 2^-18.2 of the value; 2^-17 is asked beside the codes' half step."""
     for lo, hi in ((-1.0, -0.1), (-3.0, -2.0), (-6.0, -5.0)):
         x = torch.linspace(lo, hi, 512, device="cuda").reshape(4, 128)
         codes, scale = gelu_quant(x)
