@@ -99,23 +99,30 @@ __device__ __forceinline__ void int8_place(const Int8Params& p, int t, int& m0, 
   n0 = in / gm * BN;
 }
 
-// The scales and biases of the columns n + 8 g + e, g, e = 0..3 (past N: of some column).
+// The scales and biases of the columns n + 8 g + e, g, e = 0..3 (past N: of some column). All loads of a kind behind one branch: a
+// branch a load, and each waited for the one before.
 __device__ __forceinline__ void int8_columns(const Int8Params& p, int n, float (&sb)[16], float (&bias)[16]) {
+  auto col = [&](int k) __attribute__((always_inline)) { return min(n + 2 * (k & 12) + (k & 3), p.N - 1); };
+  if (p.wide) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    if (p.wide) {
+    for (int g = 0; g < 4; ++g) {
       const float4 v = *reinterpret_cast<const float4*>(p.sb + min(n + 8 * g, p.N - 4));
       sb[4 * g] = v.x; sb[4 * g + 1] = v.y; sb[4 * g + 2] = v.z; sb[4 * g + 3] = v.w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sb[4 * g + e] = p.sb[(int64_t)min(n + 8 * g + e, p.N - 1) * p.sb_step];
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sb[k] = p.sb[(int64_t)col(k) * p.sb_step];
   }
 #pragma unroll
   for (int k = 0; k < 16; ++k) bias[k] = 0.0f;
   if (p.bias != nullptr) {
+    if (p.bias32) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) bias[k] = int8_bias(p, min(n + 2 * (k & 12) + (k & 3), p.N - 1));
+      for (int k = 0; k < 16; ++k) bias[k] = static_cast<const float*>(p.bias)[col(k)];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) bias[k] = bf16_to_f32(static_cast<const uint16_t*>(p.bias)[col(k)]);
+    }
   }
 }
 
@@ -143,6 +150,15 @@ __device__ __forceinline__ void int8_store8(const Int8Params& p, int m, int n, u
   if (p.wide) {
     if (res) o = int8_plus(o, *reinterpret_cast<const uint4*>(res));
     int8_put<false>(y, o);
+    return;
+  }
+  if (n + 8 <= p.N) {                             // at any address
+    struct __attribute__((packed, aligned(2))) V { uint32_t w[4]; };
+    if (res) {
+      const V r = *reinterpret_cast<const V*>(res);
+      o = int8_plus(o, make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]));
+    }
+    *reinterpret_cast<V*>(y) = V{{o.x, o.y, o.z, o.w}};
     return;
   }
   float a[8];
@@ -194,30 +210,30 @@ __device__ __forceinline__ void int8_epilogue(const Int8Params& p, const v16i (&
   }
 }
 
-// Any sizes and alignments: tiles of 64 (n) x 64 (m), 2 x 2 waves, 128 K bytes a stage through registers, three stages of them
-// under way, into two LDS buffers ([517, 1283] at K = 1291: 11.5 us; 22 with one stage under way). Behind K a load takes the row's
+// Any sizes and alignments: tiles of 64 T (n) x 64 T (m), 2 x 2 waves, 128 K bytes a stage through registers, stages of them under
+// way, into two LDS buffers ([517, 1283] at K = 1291, T = 1: 9.5 us; 22 with one stage under way). Behind K a load takes the row's
 // last 16 bytes, and what it should not have is dropped on the way to LDS: no load stands in a branch. SHORT: K < 16.
-constexpr int kAnyAhead = 3;
-
-template <bool SHORT>
+template <int T, bool SHORT>
 __global__ __launch_bounds__(256) void int8_any_kernel(Int8Params p) {
-  __shared__ __align__(16) uint8_t lds[2][2][64 * 128];
+  constexpr int kAhead = T == 1 ? 3 : 2, BT = 64 * T, J = 2 * T;
+  __shared__ __align__(16) uint8_t lds[2][2][BT * 128];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wn = wave & 1, wm = wave >> 1;
-  const int n0 = (int)(blockIdx.x % p.tiles_n) * 64, m0 = (int)(blockIdx.x / p.tiles_n) * 64;
+  int m0, n0;
+  int8_place<BT, BT>(p, int8_first(), m0, n0);
   const int c16 = 16 * (tid & 7), stages = (p.K + 127) >> 7;
-  const int8_t* g[2][2];                          // b's and a's rows tid / 8 and 32 + tid / 8 (past the last: that one again)
+  const int8_t* g[2][J];                          // b's and a's rows 32 j + tid / 8 (past the last: that one again)
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < J; ++j) {
     g[0][j] = p.b + (int64_t)min(n0 + 32 * j + (tid >> 3), p.N - 1) * p.bs;
     g[1][j] = p.a + (int64_t)min(m0 + 32 * j + (tid >> 3), p.M - 1) * p.as;
   }
-  uint4 v[kAnyAhead][2][2];
+  uint4 v[kAhead][2][J];
   auto load = [&](int s, auto uc) __attribute__((always_inline)) {
     constexpr int u = decltype(uc)::value;
 #pragma unroll
     for (int o = 0; o < 2; ++o)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < J; ++j) {
         if constexpr (SHORT) {
           uint8_t byte[16] = {};
           for (int k = 0; k < p.K; ++k)
@@ -228,34 +244,51 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Params p) {
         }
       }
   };
-  v16i acc[2] = {};
-  each_up<kAnyAhead>([&](auto u) __attribute__((always_inline)) { load(decltype(u)::value, u); });
-  for (int s0 = 0; s0 < stages; s0 += kAnyAhead)
-    each_up<kAnyAhead>([&](auto uc) __attribute__((always_inline)) {
-      constexpr int u = decltype(uc)::value;
-      const int s = s0 + u, buf = s & 1;
-      if (s < stages) {                           // uniform
-        if (!SHORT && s == stages - 1) {
+  v16i acc[T == 1 ? 2 : 1][T][T] = {};            // one block a wave: two sums, so that a product does not wait for the one before
+  auto step = [&](int s, auto uc, bool last) __attribute__((always_inline)) {
+    constexpr int u = decltype(uc)::value;
+    const int buf = s & 1;
+    if (!SHORT && last) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[u][j >> 1][j & 1] = drop_bytes(v[u][j >> 1][j & 1], max(128 * s + c16 - (p.K - 16), 0));
-        }
+      for (int j = 0; j < 2 * J; ++j) v[u][j / J][j % J] = drop_bytes(v[u][j / J][j % J], max(128 * s + c16 - (p.K - 16), 0));
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<uint4*>(&lds[buf][j >> 1][swz(32 * (j & 1) + (tid >> 3), tid & 7)]) = v[u][j >> 1][j & 1];
-        __syncthreads();                          // stage s is there, and every wave is done with stage s - 1
-        load(s + kAnyAhead, uc);
+    for (int j = 0; j < 2 * J; ++j)
+      *reinterpret_cast<uint4*>(&lds[buf][j / J][swz(32 * (j % J) + (tid >> 3), tid & 7)]) = v[u][j / J][j % J];
+    __syncthreads();                              // stage s is there, and every wave is done with stage s - 1
+    load(s + kAhead, uc);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {             // 16-byte chunks 4 (q / 2) + 2 (lane / 32) + q % 2 of the row
-          const int c = 4 * (q >> 1) + 2 * (lane >> 5) + (q & 1);
-          const v4i fb = *reinterpret_cast<const v4i*>(&lds[buf][0][swz(32 * wn + (lane & 31), c)]);
-          const v4i fa = *reinterpret_cast<const v4i*>(&lds[buf][1][swz(32 * wm + (lane & 31), c)]);
-          acc[q & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb, fa, acc[q & 1], 0, 0, 0);
-        }
+    for (int q = 0; q < 4; ++q) {                 // 16-byte chunks 4 (q / 2) + 2 (lane / 32) + q % 2 of the row
+      const int c = 4 * (q >> 1) + 2 * (lane >> 5) + (q & 1);
+      v4i fb[T], fa[T];
+#pragma unroll
+      for (int i = 0; i < T; ++i) {
+        fb[i] = *reinterpret_cast<const v4i*>(&lds[buf][0][swz(32 * (T * wn + i) + (lane & 31), c)]);
+        fa[i] = *reinterpret_cast<const v4i*>(&lds[buf][1][swz(32 * (T * wm + i) + (lane & 31), c)]);
       }
-    });
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+          v16i& sum = acc[T == 1 ? q & 1 : 0][i][j];
+          sum = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[i], fa[j], sum, 0, 0, 0);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // Whole rounds of kAhead stages without a branch between their loads, which would make the compiler wait for loads of the later
+  // stages too; then the last ones.
+  each_up<kAhead>([&](auto u) __attribute__((always_inline)) { load(decltype(u)::value, u); });
+  int s = 0;
+  for (; s + kAhead < stages; s += kAhead)
+    each_up<kAhead>([&](auto uc) __attribute__((always_inline)) { step(s + decltype(uc)::value, uc, false); });
+  each_up<kAhead>([&](auto uc) __attribute__((always_inline)) {
+    constexpr int u = decltype(uc)::value;
+    if (s + u < stages) step(s + u, uc, s + u == stages - 1);
+  });
   __syncthreads();                                // the epilogue overwrites the stages
-  v16i sum[1][1] = {acc[0] + acc[1]};
-  int8_epilogue<2, 2, 1, 1>(p, sum, &lds[0][0][0], m0, n0, wave, lane);
+  if constexpr (T == 1) acc[0][0][0] += acc[1][0][0];
+  int8_epilogue<2, 2, T, T>(p, acc[0], &lds[0][0][0], m0, n0, wave, lane);
 }
 
 template <int WN, int WM, int TN, int TM, int NST, bool TAIL>
@@ -692,6 +725,26 @@ __global__ __launch_bounds__(64 * kFewWaves) void int8_few_kernel(Int8Params p) 
       }
   }
   __syncthreads();
+  // The scales, biases and residual of this thread's outputs (below), under way during the products.
+  const int l = threadIdx.x, m = l & 15, n = n0 + 4 * (l >> 4);
+  float sb[4], bias[4] = {}, res[4];
+  if (l < 64) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sb[e] = p.sb[(int64_t)min(n + e, p.N - 1) * p.sb_step];
+    if (p.bias != nullptr) {
+      if (p.bias32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bias[e] = static_cast<const float*>(p.bias)[min(n + e, p.N - 1)];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bias[e] = bf16_to_f32(static_cast<const uint16_t*>(p.bias)[min(n + e, p.N - 1)]);
+      }
+    }
+    if (p.res != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) res[e] = bf16_to_f32(p.res[min(m, p.M - 1) * p.rs + min(n + e, p.N - 1)]);
+    }
+  }
   const uint8_t* const a = rows + min(row, p.M - 1) * ld + 32 * q;
   v4i acc[2] = {};
   for (int k0 = wave; k0 < blocks; k0 += kFewWaves * kFewAhead) {
@@ -709,7 +762,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void int8_few_kernel(Int8Params p) 
   *reinterpret_cast<v4i*>(sums + (wave * 64 + lane) * 4) = acc[0] + acc[1];
   __syncthreads();
   // Four outputs a thread: columns 4 (l / 16) + 0..3 of row l % 16 lie at l.
-  const int l = threadIdx.x, m = l & 15, n = n0 + 4 * (l >> 4);
   if (l >= 64 || m >= p.M) return;
   v4i s = *reinterpret_cast<const v4i*>(sums + l * 4);
 #pragma unroll
@@ -719,8 +771,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void int8_few_kernel(Int8Params p) 
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (n + e >= p.N) break;
-    float v = int8_value(s[e], sa, p.sb[(int64_t)(n + e) * p.sb_step], int8_bias(p, n + e));
-    if (p.res) v = round_bf16(v) + bf16_to_f32(p.res[m * p.rs + n + e]);
+    float v = int8_value(s[e], sa, sb[e], bias[e]);
+    if (p.res) v = round_bf16(v) + res[e];
     y[e] = (uint16_t)f32_to_bf16_bits(v);
   }
 }
@@ -789,6 +841,16 @@ static Int8Kernel kernel_of(const Int8Params& p) {
   return tile_of<4, 2, 1, 2, 2>(tail);
 }
 
+// Any alignment: tiles of 128 x 128 where there are three of 64 x 64 a compute unit and a tile is not mostly empty (us, on 64 / 128:
+// [1000, 2000] at K = 1291 15.5 / 19.8, [1500, 2000] 21.3 / 20.3, [2000, 2000] at K = 2001 35 / 27, [8191, 3391] at K = 1279 176 / 121,
+// [30, 50257] there 27.8 / 30.4).
+static Int8Kernel any_of(const Int8Params& p) {
+  const int64_t tiles = (((int64_t)p.N + 63) / 64) * (((int64_t)p.M + 63) / 64);
+  if (p.K < 16) return {reinterpret_cast<const void*>(&int8_any_kernel<1, true>), 64, 64, 256, false};
+  if (tiles < 3 * compute_units() || std::min(p.M, p.N) <= 64) return {reinterpret_cast<const void*>(&int8_any_kernel<1, false>), 64, 64, 256, false};
+  return {reinterpret_cast<const void*>(&int8_any_kernel<2, false>), 128, 128, 256, false};
+}
+
 // p.x set: the rows are quantised by the few-row kernel (few() holds, 16-byte rows of x, K % 16 == 0).
 static int int8_mm(Int8Params p, int64_t M, int64_t N, int64_t K, int64_t sa_count, int64_t sb_count, int bias_dtype, hipStream_t s,
                    const char* name) {
@@ -825,8 +887,7 @@ static int int8_mm(Int8Params p, int64_t M, int64_t N, int64_t K, int64_t sa_cou
   }
   p.wide = N % 8 == 0 && p.sb_step == 1 && std::max(p.ys, p.rs) < 1 << 25 && (uintptr_t)p.sb % 16 == 0 && on16(p.y, 2 * p.ys, M) &&
            (p.res == nullptr || on16(p.res, 2 * p.rs, M));
-  const Int8Kernel k = vector ? kernel_of(p) : Int8Kernel{K < 16 ? reinterpret_cast<const void*>(&int8_any_kernel<true>) : reinterpret_cast<const void*>(&int8_any_kernel<false>),
-                                                       64, 64, 256, false};
+  const Int8Kernel k = vector ? kernel_of(p) : any_of(p);
   const int64_t tiles_n = (N + k.bn - 1) / k.bn, tiles_m = (M + k.bm - 1) / k.bm;
   FLW_REQUIRE(k.persistent ? tiles_n * tiles_m <= 0x3FFFFFFFll : tiles_n * tiles_m * k.threads <= 0xFFFFFFFFll, FLW_E_UNSUPPORTED,
               "too many output tiles");         // a launch holds fewer than 2^32 threads
