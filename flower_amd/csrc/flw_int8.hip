@@ -174,7 +174,16 @@ template <int WN, int WM, int TN, int TM>
 __device__ __forceinline__ void int8_epilogue(const Int8Params& p, const v16i (&acc)[TN][TM], uint8_t* lds, int m0, int n0, int wave,
                                               int lane) {
   constexpr int BN = 32 * WN * TN, BM = 32 * WM * TM, NT = 64 * WN * WM, CPR = BN / 8, ROWB = 2 * BN;
-  const int wn = wave % WN, wm = wave / WN, hh = lane >> 5;
+  static_assert(NT % CPR == 0, "a thread keeps its chunk column");
+  constexpr int RPQ = NT / CPR, NQ = BM / RPQ;    // rows a pass of the stores
+  const int wn = wave % WN, wm = wave / WN, hh = lane >> 5, tid = wave * 64 + lane, ch = tid % CPR, n = n0 + 8 * ch, r0 = tid / CPR;
+  uint4 res[NQ];                                  // of wide rows, under way while the tile goes through LDS ([2048, 1280]: 11.4 -> 10.8 us)
+  const bool early = p.wide && p.res != nullptr;
+  if (early) {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+      res[q] = *reinterpret_cast<const uint4*>(p.res + (int64_t)min(m0 + RPQ * q + r0, p.M - 1) * p.rs + min(n, p.N - 8));
+  }
   float sa[TM];
 #pragma unroll
   for (int j = 0; j < TM; ++j) sa[j] = p.sa[(int64_t)min(m0 + 32 * (TM * wm + j) + (lane & 31), p.M - 1) * p.sa_step];
@@ -198,15 +207,14 @@ __device__ __forceinline__ void int8_epilogue(const Int8Params& p, const v16i (&
   }
   __builtin_amdgcn_s_waitcnt(0xC07F);             // lgkmcnt(0)
   lds_barrier();
-  static_assert(NT % CPR == 0, "a thread keeps its chunk column");
-  const int tid = wave * 64 + lane, ch = tid % CPR, n = n0 + 8 * ch;
   if (n >= p.N) return;
-#pragma unroll 4
-  for (int q = 0; q < BM * CPR / NT; ++q) {
-    const int r = (q * NT + tid) / CPR, m = m0 + r;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int r = RPQ * q + r0, m = m0 + r;
     if (m >= p.M) break;
     const uint4 o = *reinterpret_cast<const uint4*>(lds + r * ROWB + 16 * (ch ^ (r & (CPR - 1))));
-    int8_store8(p, m, n, o);
+    if (early) int8_put<false>(p.y + (int64_t)m * p.ys + n, int8_plus(o, res[q]));
+    else int8_store8(p, m, n, o);
   }
 }
 
