@@ -984,6 +984,77 @@ std::tuple<OptTensor, OptTensor, OptTensor> int8_linear_bwd(const Tensor& g0, co
   return {dx, dw, db};
 }
 
+// y = int8_linear(x, the weight's int8 rows) differentiable in x, weight, bias and residual; codes, cols: the weight's int8 and e4m3
+// codes and scales, made here when they are needed if not given. fp8: the e4m3 gradient products, which take widths in whole 16-byte
+// rows; others run in bf16. A node of its own in native code: torch's engine runs it without the interpreter (a step of 517 tokens
+// TSOLD us with the node in Python, TSNEW so).
+struct Int8LinearNode : torch::autograd::Function<Int8LinearNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                        const OptTensor& residual, const OptTensor& codes, const OptTensor& scale, const OptTensor& cols,
+                        const OptTensor& cols_scale, bool fp8, int64_t stream) {
+    ctx->save_for_backward({x, weight, cols.value_or(Tensor()), cols_scale.value_or(Tensor())});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["bias"] = bias ? (int64_t)bias->scalar_type() : -1;
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->saved_data["fp8"] = fp8;
+    ctx->saved_data["stream"] = stream;
+    return linear8(x, weight, bias, residual, codes, scale, stream);
+  }
+  static Tensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, const OptTensor& codes,
+                        const OptTensor& scale, int64_t stream) {
+    if (codes) return int8_linear(x, *codes, *scale, bias, residual, stream);
+    const auto [w8, w_scale] = quant_rows8(weight, false, stream);
+    return int8_linear(x, w8, w_scale, bias, residual, stream);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(10);
+    const Tensor& g = grads[0];
+    if (!g.defined()) return out;
+    if (c10::GradMode::is_enabled()) throw std::runtime_error("an int8 linear has no second derivative: take its gradient without create_graph");
+    refuse_tangent("an int8 linear's gradient", g);
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1];
+    const int64_t N = weight.size(0), K = weight.size(1), bias_type = ctx->saved_data["bias"].toInt();
+    const bool has_res = ctx->saved_data["residual"].toBool();
+    // the engine numbers the tensors that were given
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bias_type >= 0 && ctx->needs_input_grad(2);
+    if (has_res && ctx->needs_input_grad(bias_type >= 0 ? 3 : 2)) out[3] = g;
+    const auto type_b = (at::ScalarType)(bias_type >= 0 ? bias_type : 0);
+    if (g.numel() == 0) {
+      if (need_x) out[0] = at::zeros_like(x);
+      if (need_w) out[1] = at::zeros_like(weight);
+      if (need_b) out[2] = at::zeros({N}, weight.options().dtype(type_b));
+      return out;
+    }
+    const bool fp8 = ctx->saved_data["fp8"].toBool() && N % 16 == 0 && K % 16 == 0;
+    std::optional<std::pair<Tensor, Tensor>> cols;
+    if (saved[2].defined()) cols.emplace(saved[2], saved[3]);
+    auto [dx, dw, db] = int8_linear_bwd(g, x, weight, cols, fp8 && need_x, fp8 && need_w,
+                                        need_b ? std::optional<at::ScalarType>(type_b) : std::nullopt, ctx->saved_data["stream"].toInt());
+    if (!fp8 && (need_x || need_w)) {
+      const Tensor g2 = g.reshape({-1, N});
+      if (need_x) dx = at::matmul(g2, weight.to(g2.scalar_type()));
+      if (need_w) dw = at::matmul(g2.t(), x.reshape({-1, K}).to(g2.scalar_type()));
+    }
+    if (dx) out[0] = dx->view(x.sizes()).to(x.scalar_type());
+    if (dw) out[1] = dw->to(weight.scalar_type());
+    if (db) out[2] = *db;
+    return out;
+  }
+};
+
+Tensor int8_linear_train(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, const OptTensor& codes,
+                         const OptTensor& scale, const OptTensor& cols, const OptTensor& cols_scale, bool fp8, int64_t stream) {
+  refuse_tangent("an int8 linear", x);
+  refuse_tangent("an int8 linear", weight);
+  if (bias) refuse_tangent("an int8 linear", *bias);
+  if (residual) refuse_tangent("an int8 linear", *residual);
+  if (wants_backward(x) || wants_backward(weight) || (bias && wants_backward(*bias)) || (residual && wants_backward(*residual)))
+    return Int8LinearNode::apply(x, weight, bias, residual, codes, scale, cols, cols_scale, fp8, stream);
+  c10::AutoGradMode off(false);
+  return Int8LinearNode::linear8(x, weight, bias, residual, codes, scale, stream);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -1030,5 +1101,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("act_quant", &act_quant, nogil());
   m.def("int8_scaled_mm", &int8_scaled_mm, nogil());
   m.def("int8_linear", &int8_linear, nogil());
-  m.def("int8_linear_bwd", &int8_linear_bwd, nogil());
+  m.def("int8_linear_train", &int8_linear_train, nogil());
 }

@@ -23,46 +23,11 @@ def quantize_weight_int8(weight: torch.Tensor):
     return quant_rows(weight.detach())
 
 
-class _Int8LinearFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, codes, mod):
-        native, stream = _lib.native(), _lib.stream_or_none(x)
-        w8, w_scale = native.quant_rows8(weight, False, stream) if codes is None else codes
-        ctx.save_for_backward(x, weight)
-        ctx.mod, ctx.bias_dtype = mod, None if bias is None else bias.dtype
-        return native.int8_linear(x, w8, w_scale, bias, residual, stream)
-
-    @staticmethod
-    def backward(ctx, g):
-        x, weight = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        (N, K), mod = weight.shape, ctx.mod
-        gx = gw = gb = None
-        if g.numel() == 0:
-            gx = torch.zeros_like(x) if need_x else None
-            gw = torch.zeros_like(weight) if need_w else None
-            gb = weight.new_zeros(N, dtype=ctx.bias_dtype) if need_b else None
-            return gx, gw, gb, (g if need_r else None), None, None
-        # The e4m3 products take widths in whole 16-byte rows and the types that the casts read; others, and a module that asks
-        # for it, run in bf16.
-        fp8 = N % 16 == 0 and K % 16 == 0 and (mod is None or mod.backward_fp8)
-        cols = mod.weight_col_codes() if fp8 and need_x and mod is not None else None
-        gx, gw, gb = _lib.native().int8_linear_bwd(g, x, weight, cols, fp8 and need_x, fp8 and need_w, ctx.bias_dtype if need_b else None,
-                                                   _lib.stream_or_none(x))
-        if not fp8:
-            g2 = g.reshape(-1, N)
-            gx = g2 @ weight.to(g2.dtype) if need_x else None
-            gw = g2.t() @ x.reshape(-1, K).to(g2.dtype) if need_w else None
-        gx = gx.view(x.shape).to(x.dtype) if gx is not None else None
-        gw = gw.to(weight.dtype) if gw is not None else None
-        return gx, gw, gb, (g if need_r else None), None, None
-
-
 def int8_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                       residual: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight^T + bias``, plus ``residual``, in int8: both operands quantised now, a scale a token and a channel; bf16 out.
-    x (.., K), weight (N, K) and bias (N,) bf16 or fp32, residual bf16. Differentiable, as ``Int8Linear`` is."""
-    return _Int8LinearFn.apply(x, weight, bias, residual, None, None)
+    x (.., K), weight (N, K) and bias (N,) bf16 or fp32, residual bf16. Differentiable once by backward, as ``Int8Linear`` is."""
+    return _lib.native().int8_linear_train(x, weight, bias, residual, None, None, None, None, True, _lib.stream_or_none(x))
 
 
 class Int8Linear(Fp8Linear):
@@ -102,7 +67,12 @@ class Int8Linear(Fp8Linear):
             x = x.to(torch.get_autocast_dtype("cuda"))
         elif x.dtype not in (torch.bfloat16, torch.float32):
             x = x.to(torch.bfloat16)
-        return _Int8LinearFn.apply(x, self.weight, self.bias, residual, (w8, w_scale), self)
+        cols = (None, None)
+        if (getattr(self, "_fp8_cached", None) is not None and self.backward_fp8 and torch.is_grad_enabled() and x.requires_grad
+                and self.in_features % 16 == 0 and self.out_features % 16 == 0):
+            cols = self.weight_col_codes()              # kept for the cache's length; without one the backward makes its own
+        return _lib.native().int8_linear_train(x, self.weight, self.bias, residual, w8, w_scale, *cols, self.backward_fp8,
+                                               _lib.stream_or_none(x))
 
     def forward(self, x: torch.Tensor, x_amax=None, residual=None) -> torch.Tensor:
         return self.forward_with(x, *self.weight_codes(), residual=residual)

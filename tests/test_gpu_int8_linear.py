@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from flower_amd import _lib, int8
 from flower_amd.kernels import int8_linear, quant_rows
@@ -135,6 +136,42 @@ def test_column_sums(rows, cols, stride):
             _lib.check(lib.flw_col_sum(x.data_ptr(), rows, cols, stride, o.data_ptr(), code, ws.data_ptr(), ws.numel(), _lib.stream_of(x)), "sum")
         assert torch.equal(out[0], out[1]) and (out[:, cols] == 7).all()
         assert ((out[0, :cols].double() - want).abs() <= want.abs() * half + total * 54 * 2.0 ** -24 * (1 + half)).all()
+
+
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (3,), (0, 2), (1, 3), (2, 3)])
+@pytest.mark.parametrize("K", [64, 40])
+def test_gradients_that_are_asked_for(which, K):
+    """Any of the inputs alone, with and without a bias and a residual before it in the call: as in the call for all of them."""
+    x, w, b, g = tensors(33, 48, K)
+    given = [x, w, b, seeded((33, 48), 6, torch.bfloat16)]
+    leaves = [t.clone().requires_grad_() for t in given]
+    want = torch.autograd.grad(int8.int8_linear_train(*leaves), leaves, g)
+    some = [t.clone().requires_grad_(i in which) for i, t in enumerate(given)]
+    y = int8.int8_linear_train(*some)
+    for got, i in zip(torch.autograd.grad(y, [some[i] for i in which], g), which):
+        assert torch.equal(got, want[i])
+    # all require gradients, some are taken
+    got = torch.autograd.grad(int8.int8_linear_train(*leaves), [leaves[i] for i in which], g)
+    assert all(torch.equal(got[n], want[i]) for n, i in enumerate(which))
+    if 2 not in which:
+        some = [t.clone().requires_grad_(i in which) for i, t in enumerate(given)]
+        y = int8.int8_linear_train(some[0], some[1], None, some[3])
+        for got, i in zip(torch.autograd.grad(y, [some[i] for i in which], g), which):
+            assert torch.equal(got, want[i])
+
+
+def test_second_derivatives_and_tangents_are_refused():
+    x, w, b, g = tensors(3, 16, 16)
+    x.requires_grad_()
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(int8.int8_linear_train(x, w), x, g, create_graph=True)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        int8.int8_linear_train(forward_ad.make_dual(x.detach(), x.detach()), w)
+    y = int8.int8_linear_train(x, w.requires_grad_())
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(g)
 
 
 def test_empty_batch():
