@@ -172,6 +172,7 @@ SIGNATURES = {
     "flw_rows8_gelu": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
     "flw_rows8_swiglu": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64,
                                  c_void_p, c_void_p]),
+    "flw_quant_cols_e4m3_several": (c_int, [c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "flw_col_sum_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "flw_col_sum": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "flw_int8_scaled_mm": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,

@@ -459,14 +459,14 @@ __device__ __forceinline__ void load_tile8(const T* x, int64_t rows, int64_t col
   }
 }
 
+// (bx, by): the tile, of nbx x nby.
 template <typename T, bool TENSOR>
-__global__ __launch_bounds__(kThreads) void cols_amax_kernel(const T* __restrict__ x, int64_t rows,
-                                                             int64_t cols, int64_t rs,
-                                                             uint32_t* __restrict__ partials) {
+__device__ __forceinline__ void cols_amax_tile(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs,
+                                               uint32_t* __restrict__ partials, int bx, int by, int nbx) {
   __shared__ uint32_t red[kThreads / 8][kCT + 1];
   const int t = threadIdx.x, cg = t & 7, rg = t >> 3;
-  const int64_t c0 = (int64_t)blockIdx.x * kCT + 8 * cg;
-  const int64_t r0 = (int64_t)blockIdx.y * kRT + 8 * rg;
+  const int64_t c0 = (int64_t)bx * kCT + 8 * cg;
+  const int64_t r0 = (int64_t)by * kRT + 8 * rg;
   float f[8][8];
   load_tile8(x, rows, cols, rs, r0, c0, f);
 #pragma unroll
@@ -482,25 +482,30 @@ __global__ __launch_bounds__(kThreads) void cols_amax_kernel(const T* __restrict
     for (int g = 0; g < kThreads / 8; ++g) m = m > red[g][t] ? m : red[g][t];
     if (TENSOR) {
       m = wave_max_u32(m);
-      if (t == 0) partials[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = m;
-    } else if ((int64_t)blockIdx.x * kCT + t < cols) {
-      partials[(int64_t)blockIdx.y * cols + (int64_t)blockIdx.x * kCT + t] = m;
+      if (t == 0) partials[(int64_t)by * nbx + bx] = m;
+    } else if ((int64_t)bx * kCT + t < cols) {
+      partials[(int64_t)by * cols + (int64_t)bx * kCT + t] = m;
     }
   }
 }
 
 template <typename T, bool TENSOR>
-__global__ __launch_bounds__(kThreads) void cols_quant_t_kernel(const T* __restrict__ x, int64_t rows,
-                                                                int64_t cols, int64_t rs,
-                                                                const uint32_t* __restrict__ partials,
-                                                                int64_t nchunks, int64_t ncb,
-                                                                uint8_t* __restrict__ out, int64_t ld,
-                                                                float* __restrict__ scale_out) {
+__global__ __launch_bounds__(kThreads) void cols_amax_kernel(const T* __restrict__ x, int64_t rows,
+                                                             int64_t cols, int64_t rs,
+                                                             uint32_t* __restrict__ partials) {
+  cols_amax_tile<T, TENSOR>(x, rows, cols, rs, partials, blockIdx.x, blockIdx.y, gridDim.x);
+}
+
+template <typename T, bool TENSOR>
+__device__ __forceinline__ void cols_quant_t_tile(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs,
+                                                  const uint32_t* __restrict__ partials, int64_t nchunks, int64_t ncb,
+                                                  uint8_t* __restrict__ out, int64_t ld, float* __restrict__ scale_out,
+                                                  int bx, int by) {
   __shared__ __align__(16) uint8_t lt[kCT * kCTStride];
   __shared__ float sc[kCT], rc[kCT];
   __shared__ uint32_t red[kThreads / 64];
   const int t = threadIdx.x, cg = t & 7, rg = t >> 3;
-  const int64_t cb0 = (int64_t)blockIdx.x * kCT;
+  const int64_t cb0 = (int64_t)bx * kCT;
   // Scales of this tile's columns.
   if (TENSOR) {
     uint32_t m = 0;
@@ -509,7 +514,7 @@ __global__ __launch_bounds__(kThreads) void cols_quant_t_kernel(const T* __restr
     const float amax = __uint_as_float(m);
     const float s = (amax < kEps ? kEps : amax) / kE4m3Max;
     if (t < kCT) { sc[t] = s; rc[t] = 1.0f / s; }
-    if (blockIdx.x == 0 && blockIdx.y == 0 && t == 0) scale_out[0] = s;
+    if (bx == 0 && by == 0 && t == 0) scale_out[0] = s;
   } else {
     // Fold the column partials with all 256 threads (4 row-chunk lanes per column, several loads
     // in flight each): a single thread per column walking the chunks serialises their latency.
@@ -534,13 +539,13 @@ __global__ __launch_bounds__(kThreads) void cols_quant_t_kernel(const T* __restr
       s = s < kEps ? kEps : s;
       sc[t] = s;
       rc[t] = 1.0f / s;
-      if (blockIdx.y == 0 && c < cols) scale_out[c] = s;
+      if (by == 0 && c < cols) scale_out[c] = s;
     }
   }
   __syncthreads();
 
   const int64_t c0 = cb0 + 8 * cg;
-  const int64_t r0 = (int64_t)blockIdx.y * kRT + 8 * rg;
+  const int64_t r0 = (int64_t)by * kRT + 8 * rg;
   float f[8][8];
   load_tile8(x, rows, cols, rs, r0, c0, f);
 #pragma unroll
@@ -576,7 +581,7 @@ __global__ __launch_bounds__(kThreads) void cols_quant_t_kernel(const T* __restr
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int rr = 64 * q + 16 * part;
-      const int64_t r = (int64_t)blockIdx.y * kRT + rr;
+      const int64_t r = (int64_t)by * kRT + rr;
       if (r < ld) {
         const uint2 a = *reinterpret_cast<const uint2*>(lt + cl * kCTStride + rr);
         const uint2 b = *reinterpret_cast<const uint2*>(lt + cl * kCTStride + rr + 8);
@@ -584,6 +589,46 @@ __global__ __launch_bounds__(kThreads) void cols_quant_t_kernel(const T* __restr
       }
     }
   }
+}
+
+template <typename T, bool TENSOR>
+__global__ __launch_bounds__(kThreads) void cols_quant_t_kernel(const T* __restrict__ x, int64_t rows,
+                                                                int64_t cols, int64_t rs,
+                                                                const uint32_t* __restrict__ partials,
+                                                                int64_t nchunks, int64_t ncb,
+                                                                uint8_t* __restrict__ out, int64_t ld,
+                                                                float* __restrict__ scale_out) {
+  cols_quant_t_tile<T, TENSOR>(x, rows, cols, rs, partials, nchunks, ncb, out, ld, scale_out, blockIdx.x, blockIdx.y);
+}
+
+// The per-column cast of up to three bf16 matrices in the same two launches: a small training step's casts are launches more than
+// work (the step of 517 rows through an int8 linear [1280, 1280] and back 47 us on the GPU so, 64 with one cast after the other).
+constexpr int kMostJobs = 3;
+struct ColsJobs {
+  const uint16_t* x[kMostJobs];
+  int64_t rows[kMostJobs], cols[kMostJobs], rs[kMostJobs], ld[kMostJobs];
+  uint32_t* part[kMostJobs];
+  uint8_t* out[kMostJobs];
+  float* scale[kMostJobs];
+  int ncb[kMostJobs], nchunks[kMostJobs];
+  unsigned amax_end[kMostJobs], quant_end[kMostJobs];      // workgroups of this matrix and those before it (past the last: all ones)
+};
+__device__ __forceinline__ int job_of(const unsigned (&end)[kMostJobs], unsigned& b) {
+  int k = 0;
+  while (k < kMostJobs - 1 && b >= end[k]) ++k;
+  if (k > 0) b -= end[k - 1];
+  return k;
+}
+__global__ __launch_bounds__(kThreads) void cols_amax_several_kernel(ColsJobs p) {
+  unsigned b = blockIdx.x;
+  const int k = job_of(p.amax_end, b);
+  cols_amax_tile<uint16_t, false>(p.x[k], p.rows[k], p.cols[k], p.rs[k], p.part[k], b % p.ncb[k], b / p.ncb[k], p.ncb[k]);
+}
+__global__ __launch_bounds__(kThreads) void cols_quant_t_several_kernel(ColsJobs p) {
+  unsigned b = blockIdx.x;
+  const int k = job_of(p.quant_end, b);
+  cols_quant_t_tile<uint16_t, false>(p.x[k], p.rows[k], p.cols[k], p.rs[k], p.part[k], p.nchunks[k], p.ncb[k], p.out[k], p.ld[k], p.scale[k],
+                                     b % p.ncb[k], b / p.ncb[k]);
 }
 
 // ---------------------------------------------------------------- activation + per-row quantiser
@@ -992,6 +1037,39 @@ extern "C" int flw_fake_quant_e4m3(const void* x, int dtype, int64_t B, int64_t 
   p.d0 = B; p.d1 = H; p.d2 = T; p.d3 = D;
   p.nchunks = nchunks_of(T); p.partials = static_cast<uint32_t*>(workspace); p.granularity = granularity;
   return launch_quant<1>(p, 1, dtype, static_cast<hipStream_t>(stream), "flw_fake_quant_e4m3", take_timer());
+}
+
+extern "C" int flw_quant_cols_e4m3_several(const flw_cols_job* jobs, int count, void* workspace, size_t workspace_bytes, void* stream) {
+  FLW_REQUIRE(jobs != nullptr && count >= 1 && count <= kMostJobs, FLW_E_INVALID, "between 1 and %d matrices, got %d", kMostJobs, count);
+  ColsJobs p{};
+  size_t need = 0;
+  int64_t g1 = 0, g2 = 0;
+  for (int k = 0; k < count; ++k) {
+    const flw_cols_job& j = jobs[k];
+    FLW_REQUIRE(j.x != nullptr && j.out_t != nullptr && j.scale_out != nullptr, FLW_E_INVALID, "null pointer");
+    FLW_REQUIRE(j.rows > 0 && j.cols > 0, FLW_E_INVALID, "empty matrix");
+    FLW_REQUIRE(j.cols % 8 == 0 && j.row_stride % 8 == 0 && j.row_stride >= j.cols && ((uintptr_t)j.x & 15) == 0, FLW_E_INVALID,
+                "cols and row_stride must be multiples of 8, rows 16-byte aligned");
+    FLW_REQUIRE(j.ld >= j.rows && j.ld % 16 == 0 && ((uintptr_t)j.out_t & 15) == 0, FLW_E_INVALID,
+                "ld must be >= rows and a multiple of 16, out_t 16-byte aligned");
+    const int64_t nchunks = (j.rows + kRT - 1) / kRT, ncb = (j.cols + kCT - 1) / kCT, oy = (j.ld + kRT - 1) / kRT;
+    FLW_REQUIRE(ncb <= 0x7FFFFF && oy <= 0x7FFFFF && (g2 += ncb * oy) * kThreads <= 0xFFFFFFFFll, FLW_E_UNSUPPORTED, "matrices too large");
+    g1 += ncb * nchunks;
+    p.x[k] = static_cast<const uint16_t*>(j.x);
+    p.rows[k] = j.rows; p.cols[k] = j.cols; p.rs[k] = j.row_stride; p.ld[k] = j.ld;
+    p.part[k] = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + need);
+    p.out[k] = j.out_t; p.scale[k] = j.scale_out;
+    p.ncb[k] = (int)ncb; p.nchunks[k] = (int)nchunks;
+    p.amax_end[k] = (unsigned)g1; p.quant_end[k] = (unsigned)g2;
+    need += flw_quant_cols_workspace_bytes(j.rows, j.cols);
+  }
+  for (int k = count; k < kMostJobs; ++k) p.amax_end[k] = p.quant_end[k] = 0xFFFFFFFFu;
+  FLW_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 4 == 0 && workspace_bytes >= need, FLW_E_WORKSPACE, "workspace needs %zu bytes", need);
+  const Timer tm = take_timer();
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  (void)launch_ext(reinterpret_cast<const void*>(&cols_amax_several_kernel), dim3((unsigned)g1), dim3(kThreads), 0, s, p, tm.start, nullptr);
+  (void)launch_ext(reinterpret_cast<const void*>(&cols_quant_t_several_kernel), dim3((unsigned)g2), dim3(kThreads), 0, s, p, nullptr, tm.stop);
+  return check_launch("flw_quant_cols_e4m3_several");
 }
 
 template <int ACT>

@@ -949,7 +949,7 @@ Tensor int8_linear(const Tensor& x0, const Tensor& b0, const Tensor& b_scale, co
 // The gradients of y = x W^T (+ bias) straight through its quantisers, from g = dy: (dx, dW, db), each when asked for. The products
 // are the e4m3 ones of the rowwise recipe: g by rows with W by columns (w_cols: its codes transposed and scales, made here if not
 // given), and g by columns with x by columns, the token axis padded with zeros to a multiple of 128. N and K are multiples of 16.
-// All of it in one call: a small step's fourteen launches take less time than as many calls from Python.
+// All of it in one call: a small step's ten launches take less time than as many calls from Python.
 std::tuple<OptTensor, OptTensor, OptTensor> int8_linear_bwd(const Tensor& g0, const Tensor& x0, const Tensor& weight,
                                                             const std::optional<std::pair<Tensor, Tensor>>& w_cols, bool need_x,
                                                             bool need_w, const std::optional<at::ScalarType>& bias_dtype, int64_t stream) {
@@ -963,18 +963,40 @@ std::tuple<OptTensor, OptTensor, OptTensor> int8_linear_bwd(const Tensor& g0, co
   }
   const int64_t M = g.size(0), ld = (M + 127) / 128 * 128;
   OptTensor dx, dw, db;
+  // The casts by columns (the weight's if not given, g's and x's) in one call.
+  struct Cast {
+    Tensor rows, codes, scale;
+  } w, gc, x;
+  std::vector<flw_cols_job> jobs;
+  size_t need = 0;
+  auto by_columns = [&](Cast& c, const Tensor& t, int64_t cols_ld) {
+    c.rows = vector_rows(t);
+    const int64_t R = c.rows.size(0), C = c.rows.size(1);
+    if (c.rows.scalar_type() != at::kBFloat16) {
+      std::tie(c.codes, c.scale) = quant_cols(c.rows, true, cols_ld, stream);
+      return;
+    }
+    c.codes = empty(t, {C, cols_ld}, at::kByte);
+    c.scale = empty(t, {C}, at::kFloat);
+    jobs.push_back({c.rows.data_ptr(), R, C, c.rows.stride(0), u8(c.codes), cols_ld, f32(c.scale)});
+    need += flw_quant_cols_workspace_bytes(R, C);
+  };
+  if (need_x && !w_cols) by_columns(w, weight, N);
+  if (need_w) {
+    by_columns(gc, g, ld);
+    by_columns(x, x0, ld);
+  }
+  if (!jobs.empty()) {
+    const Tensor ws = workspace(g, need);
+    check(flw_quant_cols_e4m3_several(jobs.data(), (int)jobs.size(), ws.data_ptr(), (size_t)ws.numel(), str(stream)), "int8 linear backward");
+  }
   if (need_x) {
     Rows8 rows(g, true);
     check(flw_rows8(g.data_ptr(), FLW_BF16, M, N, gs, FLW_E4M3, rows.codes.data_ptr(), N, f32(rows.scale), str(stream)),
           "int8 linear backward");
-    const auto cols = w_cols ? std::make_tuple(w_cols->first, w_cols->second) : quant_cols(vector_rows(weight), true, N, stream);
-    dx = scaled_mm(rows.codes, rows.scale, std::get<0>(cols), std::get<1>(cols), std::nullopt, true, stream);
+    dx = scaled_mm(rows.codes, rows.scale, w_cols ? w_cols->first : w.codes, w_cols ? w_cols->second : w.scale, std::nullopt, true, stream);
   }
-  if (need_w) {
-    const auto [g8, g_scale] = quant_cols(g, true, ld, stream);
-    const auto [x8, x_scale] = quant_cols(vector_rows(x0), true, ld, stream);
-    dw = scaled_mm(g8, g_scale, x8, x_scale, std::nullopt, true, stream);
-  }
+  if (need_w) dw = scaled_mm(gc.codes, gc.scale, x.codes, x.scale, std::nullopt, true, stream);
   if (bias_dtype) {
     db = empty(g, {N}, *bias_dtype == at::kFloat ? at::kFloat : at::kBFloat16);
     const Tensor ws = workspace(g, flw_col_sum_workspace_bytes(M, N));
@@ -987,7 +1009,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> int8_linear_bwd(const Tensor& g0, co
 // y = int8_linear(x, the weight's int8 rows) differentiable in x, weight, bias and residual; codes, cols: the weight's int8 and e4m3
 // codes and scales, made here when they are needed if not given. fp8: the e4m3 gradient products, which take widths in whole 16-byte
 // rows; others run in bf16. A node of its own in native code: torch's engine runs it without the interpreter (a step of 517 tokens
-// TSOLD us with the node in Python, TSNEW so).
+// 130 us with the node in Python, 70 to 110 so, by the host).
 struct Int8LinearNode : torch::autograd::Function<Int8LinearNode> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias,
                         const OptTensor& residual, const OptTensor& codes, const OptTensor& scale, const OptTensor& cols,

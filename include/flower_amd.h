@@ -273,6 +273,17 @@ int flw_quant_cols_e4m3(const void* x, int dtype, int64_t rows, int64_t cols, in
                         int granularity, uint8_t* out_t, int64_t ld, float* scale_out, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* flw_quant_cols_e4m3 (FLW_SCALE_COLUMN) of one to three bf16 matrices in its two launches: the casts of a linear's backward, whose
+ * small steps are bound by launches. workspace: the sum of the matrices' flw_quant_cols_workspace_bytes. */
+typedef struct {
+  const void* x; /* [rows, cols] bf16 */
+  int64_t rows, cols, row_stride;
+  uint8_t* out_t; /* [cols, ld] */
+  int64_t ld;
+  float* scale_out; /* [cols] */
+} flw_cols_job;
+int flw_quant_cols_e4m3_several(const flw_cols_job* jobs, int count, void* workspace, size_t workspace_bytes, void* stream);
+
 /* The tensorwise e4m3 cast of torchao Float8Linear (one scale for the whole matrix, the
  * reference's default recipe; torchao 0.18.0, not vendored, enabled at flower/train.py:368-370)
  * of a bf16 matrix x [rows, cols] written in both layouts the training GEMMs read: out8 [rows, cols]

@@ -6,6 +6,8 @@ largest is asked, as of the e4m3 linears). Against the gradient of the unquantis
 2^-4 of a value each, uniform within it, is 2^-4 / sqrt 3 * sqrt 2 = 5.1 % of the result's size at the most; 6 % is asked.
 """
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -14,11 +16,16 @@ from torch.autograd import forward_ad
 
 from flower_amd import _lib, int8
 from flower_amd.kernels import int8_linear, quant_rows
-from flower_amd.precision import fp8_weight_cache
+from flower_amd.precision import fp8_weight_cache, quantize_cols
 from oracle.gemm import fp8_linear_backward
 from tests.gpu_util import seeded, to_np
 
 pytestmark = pytest.mark.gpu
+
+
+class _Job(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("out_t", ctypes.c_void_p), ("ld", ctypes.c_int64), ("scale_out", ctypes.c_void_p)]
 
 
 def tensors(M, N, K, dtype=torch.bfloat16):
@@ -118,6 +125,21 @@ def test_gradients_of_any_layout(M, N, K):
     leaf = x.clone().requires_grad_()
     int8.int8_linear_train(leaf, w).sum(0).pow(2).sum().backward()                      # a gradient that autograd expands
     assert leaf.grad.any()
+
+
+@pytest.mark.parametrize("shapes", [[(5, 8, 16)], [(300, 136, 304), (1, 64, 16)], [(517, 1280, 640), (1280, 640, 1280), (517, 640, 768)],
+                                    [(256, 64, 256), (257, 72, 272), (600, 8, 608)]])
+def test_casts_by_columns_together(shapes):
+    """The casts of one to three matrices in one call: the bits of each one's own."""
+    lib = _lib.load()
+    xs = [seeded((r, c + 8), 20 + k, torch.bfloat16)[:, :c] for k, (r, c, _) in enumerate(shapes)]
+    outs = [(torch.full((c, ld), 7, dtype=torch.uint8, device="cuda"), torch.zeros(c, device="cuda")) for _, c, ld in shapes]
+    jobs = (_Job * 3)(*(_Job(x.data_ptr(), r, c, c + 8, o.data_ptr(), ld, s.data_ptr()) for x, (r, c, ld), (o, s) in zip(xs, shapes, outs)))
+    ws = torch.full((sum(lib.flw_quant_cols_workspace_bytes(r, c) for r, c, _ in shapes),), 255, dtype=torch.uint8, device="cuda")
+    _lib.check(lib.flw_quant_cols_e4m3_several(ctypes.byref(jobs), len(shapes), ws.data_ptr(), ws.numel(), _lib.stream_of(ws)), "several")
+    for x, (_, _, ld), (o, s) in zip(xs, shapes, outs):
+        want, scale = quantize_cols(x, "column", ld=ld)
+        assert torch.equal(o, want.view(torch.uint8)) and torch.equal(s, scale)
 
 
 @pytest.mark.parametrize("rows", [1, 3, 32, 33, 2048, 2049, 5000])

@@ -1,5 +1,7 @@
 """CPU: what the 8-bit rows and the int8 product refuse, and Int8Linear's conversion rules."""
 
+import ctypes
+
 import pytest
 import torch
 import torch.nn as nn
@@ -147,3 +149,20 @@ def test_c_entries_refuse_on_the_host():
     for change, rc in ((dict(x=None), 1), (dict(out=None), 1), (dict(rows=0), 1), (dict(cols=0), 1), (dict(xs=4), 1), (dict(dtype=3), 2), (dict(wb=19), 3),
                        (dict(ws=None), 3), (dict(ws=P + 4), 3), (dict(x=P + 1), 1), (dict(out=P + 2), 1), (dict(rows=2 ** 24, wb=2 ** 30), 2)):
         assert tot(**change) == rc, change
+
+    class Job(ctypes.Structure):
+        _fields_ = [("x", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                    ("out_t", ctypes.c_void_p), ("ld", ctypes.c_int64), ("scale_out", ctypes.c_void_p)]
+
+    size = lib.flw_quant_cols_workspace_bytes(20, 64)
+    good = dict(x=P, rows=20, cols=64, row_stride=64, out_t=P, ld=32, scale_out=P)
+
+    def casts(count=2, ws=P, wb=2 * size, **change):
+        jobs = (Job * 2)(Job(*good.values()), Job(*{**good, **change}.values()))
+        return lib.flw_quant_cols_e4m3_several(ctypes.byref(jobs), count, ws, wb, None)
+
+    for change, rc in ((dict(x=None), 1), (dict(out_t=None), 1), (dict(scale_out=None), 1), (dict(rows=0), 1), (dict(cols=0), 1), (dict(cols=60), 1),
+                       (dict(row_stride=56), 1), (dict(row_stride=68), 1), (dict(x=P + 8), 1), (dict(out_t=P + 8), 1), (dict(ld=16), 1),
+                       (dict(ld=24), 1), (dict(rows=2 ** 40, ld=2 ** 40), 2), (dict(count=0), 1), (dict(count=4), 1), (dict(ws=None), 3),
+                       (dict(wb=2 * size - 1), 3)):
+        assert casts(**change) == rc, change
