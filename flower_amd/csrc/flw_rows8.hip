@@ -9,8 +9,9 @@
 // do as flw_quant_rows_e4m3's.
 //
 // One pass over memory. A row is held by LPR lanes (64, 256 or 1024 threads), each up to four chunks of 8 values in
-// registers, between the loads, the sum of squares, the maximum and the codes; wider rows are refused. Bound by HBM for many rows, by the latency of
-// load, reduction, reduction, store for few.
+// registers, between the loads, the sum of squares, the maximum and the codes; wider rows are refused. Bound by HBM for many rows
+// ([65536, 4096] into int8: as they are 134 us, 6.0 TB/s, addition and norm 314, 6.0, SwiGLU 228, 5.9), norm alone (168, 4.8) and GELU
+// (209, 3.9) by what the vector unit issues; by the latency of load, reduction, reduction, store for few.
 #include "flw_common.h"
 
 namespace flw {

@@ -5,7 +5,8 @@
 // its autograd node and its module stay in Python, and every function takes the stream it launches on
 // (torch's current stream of the tensors' device, as a handle). The rotary positions and the paged
 // cache's operators are here as a whole, their checks and the one's autograd node too: their kernels
-// take 3 to 6 us in a decode step, less than the same checks take in Python; and so are the 8-bit rows and the int8 product.
+// take 3 to 6 us in a decode step, less than the same checks take in Python; and so are the 8-bit rows and
+// the int8 linear, with its node.
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
