@@ -1068,6 +1068,9 @@ struct Int8LinearNode : torch::autograd::Function<Int8LinearNode> {
 
 Tensor int8_linear_train(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, const OptTensor& codes,
                          const OptTensor& scale, const OptTensor& cols, const OptTensor& cols_scale, bool fp8, int64_t stream) {
+  REFUSE_UNLESS(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.device() == x.device(),
+                "an int8 linear of rows ", x.sizes(), " takes a weight (N, ", x.dim() ? x.size(-1) : 0, ") on ", x.device(), ", got ",
+                weight.sizes(), " on ", weight.device());
   refuse_tangent("an int8 linear", x);
   refuse_tangent("an int8 linear", weight);
   if (bias) refuse_tangent("an int8 linear", *bias);

@@ -84,6 +84,16 @@ def test_gradients_and_tangents_are_refused_not_dropped():
                 call()
 
 
+def test_int8_linear_train_refuses():
+    for x, w in ((X, torch.ones(5, 7)), (X, W), (torch.zeros(()), torch.ones(5, 8)), (X, torch.ones(5, 8, device="meta"))):
+        with pytest.raises(ValueError, match="takes a weight"):
+            int8.int8_linear_train(x, w)
+    with pytest.raises(RuntimeError, match="only on a ROCm GPU"):
+        int8.int8_linear_train(X, torch.ones(5, 8))
+    with pytest.raises(TypeError, match="bfloat16 or float32"):
+        int8.int8_linear_train(X, torch.ones(5, 8).half())
+
+
 class Model(nn.Module):
     def __init__(self, blocks=4):
         super().__init__()
