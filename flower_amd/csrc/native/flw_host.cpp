@@ -791,6 +791,8 @@ void check_like(const char* what, const char* name, const Tensor& t, const Tenso
   refuse_gradients(what, t);
 }
 
+constexpr int64_t kRows8Cols = 32768;     // the widest rows that flw_rows8 and its kin take
+
 // The codes (.., K) and scales (..) that a pass over the rows x writes: launch(rows, codes, scale).
 struct Rows8 {
   Tensor codes, scale;
@@ -993,7 +995,9 @@ std::tuple<OptTensor, OptTensor, OptTensor> int8_linear_bwd(const Tensor& g0, co
   }
   if (need_x) {
     Rows8 rows(g, true);
-    check(flw_rows8(g.data_ptr(), FLW_BF16, M, N, gs, FLW_E4M3, rows.codes.data_ptr(), N, f32(rows.scale), str(stream)),
+    // flw_rows8 holds a row in registers, up to kRows8Cols values; the other quantiser reads wider ones twice, for the same codes.
+    check(N <= kRows8Cols ? flw_rows8(g.data_ptr(), FLW_BF16, M, N, gs, FLW_E4M3, rows.codes.data_ptr(), N, f32(rows.scale), str(stream))
+                          : flw_quant_rows_e4m3(g.data_ptr(), FLW_BF16, M, N, gs, u8(rows.codes), f32(rows.scale), str(stream)),
           "int8 linear backward");
     dx = scaled_mm(rows.codes, rows.scale, w_cols ? w_cols->first : w.codes, w_cols ? w_cols->second : w.scale, std::nullopt, true, stream);
   }
