@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <sstream>
@@ -792,6 +793,7 @@ void check_like(const char* what, const char* name, const Tensor& t, const Tenso
 }
 
 constexpr int64_t kRows8Cols = 32768;     // the widest rows that flw_rows8 and its kin take
+constexpr int64_t kSumRows = 65535 * 128;  // the most rows of one flw_col_sum
 
 // The codes (.., K) and scales (..) that a pass over the rows x writes: launch(rows, codes, scale).
 struct Rows8 {
@@ -1003,10 +1005,21 @@ std::tuple<OptTensor, OptTensor, OptTensor> int8_linear_bwd(const Tensor& g0, co
   }
   if (need_w) dw = scaled_mm(gc.codes, gc.scale, x.codes, x.scale, std::nullopt, true, stream);
   if (bias_dtype) {
-    db = empty(g, {N}, *bias_dtype == at::kFloat ? at::kFloat : at::kBFloat16);
-    const Tensor ws = workspace(g, flw_col_sum_workspace_bytes(M, N));
-    check(flw_col_sum(g.data_ptr(), M, N, gs, db->data_ptr(), dtype_code(*db), ws.data_ptr(), (size_t)ws.numel(), str(stream)),
-          "int8 linear backward");
+    auto sum = [&](int64_t first, int64_t rows, at::ScalarType type) {
+      const Tensor out = empty(g, {N}, type);
+      const Tensor ws = workspace(g, flw_col_sum_workspace_bytes(rows, N));
+      check(flw_col_sum(static_cast<const uint16_t*>(g.data_ptr()) + first * gs, rows, N, gs, out.data_ptr(), dtype_code(out), ws.data_ptr(),
+                        (size_t)ws.numel(), str(stream)),
+            "int8 linear backward");
+      return out;
+    };
+    if (M <= kSumRows) {
+      db = sum(0, M, *bias_dtype);
+    } else {                                       // parts in fp32, added in order
+      Tensor total = sum(0, kSumRows, at::kFloat);
+      for (int64_t first = kSumRows; first < M; first += kSumRows) total.add_(sum(first, std::min(kSumRows, M - first), at::kFloat));
+      db = total.to(*bias_dtype);
+    }
   }
   return {dx, dw, db};
 }

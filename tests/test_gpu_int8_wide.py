@@ -1,4 +1,4 @@
-"""GPU: int8 linears at the ends of what they take: outputs wider than a pass over 8-bit rows.
+"""GPU: int8 linears at the ends of what they take: outputs wider than a pass over 8-bit rows, more rows than a column sum.
 
 Tolerances as in test_gpu_int8_linear.py: a gradient is off by its bf16 rounding, 2^-8, and the matrix unit's fp32 sums, a thousandth
 of the largest.
@@ -46,3 +46,23 @@ def test_a_wide_modules_input_gradient(N):
     assert torch.equal(torch.autograd.grad(mod(x), x, g)[0], want)
     with fp8_weight_cache(torch.nn.ModuleList([mod])):
         assert torch.equal(torch.autograd.grad(mod(x), x, g)[0], want)
+
+
+@pytest.mark.parametrize("rows", [65535 * 128, 65535 * 128 + 1])
+def test_gradients_of_very_many_rows(rows):
+    """More rows than one column sum takes. The bias's gradient: chains of 32 + 3 + 4096 + 16 additions in fp32 of each part, and the
+    parts', each off by 2^-24 of the absolute sum, then the rounding. Rows of the input's gradient are the same bits as alone."""
+    N = K = 16
+    rng = torch.Generator(device="cuda").manual_seed(1)
+    x, g = (torch.randn(rows, n, generator=rng, device="cuda").bfloat16() for n in (K, N))
+    w, b = seeded((N, K), 2, torch.bfloat16, scale=0.25), seeded((N,), 3, torch.bfloat16)
+    s, total = g.double().sum(0), g.abs().sum(0, dtype=torch.float64)
+    for bias in (b, b.float()):
+        leaves = [t.detach().requires_grad_() for t in (x, w, bias)]
+        gx, gw, gb = torch.autograd.grad(int8.int8_linear_train(*leaves), leaves, g)
+        half = 2.0 ** -8 if bias.dtype == torch.bfloat16 else 2.0 ** -24
+        assert gb.dtype == bias.dtype and ((gb.double() - s).abs() <= s.abs() * half + total * 4150 * 2.0 ** -24).all()
+    some = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device="cuda")
+    few = [x[some].clone().requires_grad_(), w.detach(), b.detach()]
+    assert torch.equal(gx[some], torch.autograd.grad(int8.int8_linear_train(*few), few[0], g[some])[0])
+    assert torch.isfinite(gw).all() and gw.any()
