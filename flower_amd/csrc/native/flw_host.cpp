@@ -794,6 +794,7 @@ void check_like(const char* what, const char* name, const Tensor& t, const Tenso
 
 constexpr int64_t kRows8Cols = 32768;     // the widest rows that flw_rows8 and its kin take
 constexpr int64_t kSumRows = 65535 * 128;  // the most rows of one flw_col_sum
+constexpr int64_t kCols32Rows = 65535 * 256;       // the most fp32 rows of one flw_quant_cols_e4m3
 
 // The codes (.., K) and scales (..) that a pass over the rows x writes: launch(rows, codes, scale).
 struct Rows8 {
@@ -1092,8 +1093,17 @@ Tensor int8_linear_train(const Tensor& x, const Tensor& weight, const OptTensor&
   refuse_tangent("an int8 linear", weight);
   if (bias) refuse_tangent("an int8 linear", *bias);
   if (residual) refuse_tangent("an int8 linear", *residual);
-  if (wants_backward(x) || wants_backward(weight) || (bias && wants_backward(*bias)) || (residual && wants_backward(*residual)))
+  if (wants_backward(x) || wants_backward(weight) || (bias && wants_backward(*bias)) || (residual && wants_backward(*residual))) {
+    // what the backward could not cast is refused here, not behind a good forward
+    const int64_t N = weight.size(0), K = weight.size(1);
+    if (fp8 && N % 16 == 0 && K % 16 == 0 && K > 0) {
+      auto castable = [](const Tensor& t, int64_t rows) { return t.scalar_type() != at::kFloat || rows <= kCols32Rows; };
+      REFUSE_UNLESS((!wants_backward(weight) || castable(x, x.numel() / K)) && (!wants_backward(x) || cols || castable(weight, N)),
+                    "an int8 linear's gradient casts at most ", kCols32Rows, " float32 rows of its input or weight, got ", x.numel() / K,
+                    " and ", N, ": pass bfloat16");
+    }
     return Int8LinearNode::apply(x, weight, bias, residual, codes, scale, cols, cols_scale, fp8, stream);
+  }
   c10::AutoGradMode off(false);
   return Int8LinearNode::linear8(x, weight, bias, residual, codes, scale, stream);
 }

@@ -26,7 +26,8 @@ def quantize_weight_int8(weight: torch.Tensor):
 def int8_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                       residual: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight^T + bias``, plus ``residual``, in int8: both operands quantised now, a scale a token and a channel; bf16 out.
-    x (.., K), weight (N, K) and bias (N,) bf16 or fp32, residual bf16. Differentiable once by backward, as ``Int8Linear`` is."""
+    x (.., K), weight (N, K) and bias (N,) bf16 or fp32, residual bf16; for a gradient at most 65535 * 256 fp32 rows. Differentiable
+    once by backward, as ``Int8Linear`` is."""
     return _lib.native().int8_linear_train(x, weight, bias, residual, None, None, None, None, True, _lib.stream_or_none(x))
 
 
