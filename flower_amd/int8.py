@@ -6,6 +6,8 @@
 ``int8_linear_train``     its forward as a function, differentiable in input, weight, bias and residual
 ``convert_model_to_int8`` replaces a model's linears as ``convert_model_to_fp8`` does (flower/precision.py:134-195), by the
                           same rules; ``fp8_weight_cache`` then keeps the int8 codes for the length of its block.
+
+Rows in 8 bits hold at most 32768 values (``flower_amd.kernels.quant_rows``): so many input features, and any number of outputs.
 """
 
 from __future__ import annotations
@@ -17,6 +19,8 @@ from . import _lib
 from .kernels.int8 import int8_scaled_mm, quant_rows
 from .precision import Fp8Linear, fp8_module_filter, quantize_weight_cols
 
+MAX_IN_FEATURES = 32768
+
 
 def quantize_weight_int8(weight: torch.Tensor):
     """(codes (N, K) int8, scale (N,) float32) of a weight: one scale an output channel."""
@@ -26,22 +30,29 @@ def quantize_weight_int8(weight: torch.Tensor):
 def int8_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                       residual: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight^T + bias``, plus ``residual``, in int8: both operands quantised now, a scale a token and a channel; bf16 out.
-    x (.., K), weight (N, K) and bias (N,) bf16 or fp32, residual bf16; for a gradient at most 65535 * 256 fp32 rows. Differentiable
-    once by backward, as ``Int8Linear`` is."""
+    x (.., K), K <= 32768, weight (N, K) and bias (N,) bf16 or fp32, residual bf16; for a gradient at most 65535 * 256 fp32 rows.
+    Differentiable once by backward, as ``Int8Linear`` is."""
     return _lib.native().int8_linear_train(x, weight, bias, residual, None, None, None, None, True, _lib.stream_or_none(x))
+
+
+def _check_width(in_features: int) -> None:
+    if in_features > MAX_IN_FEATURES:
+        raise ValueError(f"an Int8Linear takes at most {MAX_IN_FEATURES} input features, got {in_features}")
 
 
 class Int8Linear(Fp8Linear):
     """``nn.Linear`` in int8 (see the module). Shares the Parameters of the Linear it was built from. The weight is quantised
-    on every call unless an ``fp8_weight_cache`` is active. ``forward_codes`` takes the input as codes and scales already, from
-    ``rms_norm_quant`` or another of the passes of ``flower_amd.kernels``."""
+    on every call unless an ``fp8_weight_cache`` is active. At most 32768 input features. ``forward_codes`` takes the input as
+    codes and scales already, from ``rms_norm_quant`` or another of the passes of ``flower_amd.kernels``."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None) -> None:
+        _check_width(in_features)
         super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
         self.recipe = "int8"
 
     @classmethod
     def from_linear(cls, lin: nn.Linear) -> "Int8Linear":
+        _check_width(lin.in_features)
         new = super().from_linear(lin)
         new.recipe = "int8"
         return new
@@ -85,15 +96,15 @@ class Int8Linear(Fp8Linear):
 
 
 def convert_model_to_int8(model: nn.Module, *, keep_bf16_blocks: int = 1, verbose: bool = True):
-    """Replace every Linear that ``fp8_module_filter`` admits by an ``Int8Linear`` sharing its Parameters, in place; returns
-    (model, info). As ``convert_model_to_fp8``, it refuses a model without ``blocks``."""
+    """Replace every Linear that ``fp8_module_filter`` admits, of at most 32768 input features, by an ``Int8Linear`` sharing its
+    Parameters, in place; returns (model, info). As ``convert_model_to_fp8``, it refuses a model without ``blocks``."""
     num_layers = len(getattr(model, "blocks", []))
     if num_layers == 0:
         raise RuntimeError("convert_model_to_int8 found no `blocks` on the model; the block-range guardrail cannot be applied. "
                            "Refusing to convert blindly.")
     admit = fp8_module_filter(num_layers, keep_bf16_blocks)
     named = list(model.named_modules())
-    targets = [(fqn, m) for fqn, m in named if admit(m, fqn)]
+    targets = [(fqn, m) for fqn, m in named if admit(m, fqn) and m.in_features <= MAX_IN_FEATURES]
     for fqn, mod in targets:
         owner, _, attr = fqn.rpartition(".")
         setattr(model.get_submodule(owner) if owner else model, attr, Int8Linear.from_linear(mod))

@@ -1,7 +1,9 @@
-"""CPU: what an int8 linear's training takes, refused before its forward rather than behind it."""
+"""CPU: what an int8 linear's training takes, refused before its forward rather than behind it, and which linears are
+converted."""
 
 import pytest
 import torch
+import torch.nn as nn
 
 from flower_amd import int8
 
@@ -21,3 +23,17 @@ def test_float32_rows_that_the_backward_cannot_cast_are_refused_at_once():
                  (many[:, :8], leaf(w[:, :8])), (many, w)):
         with pytest.raises(RuntimeError, match="only on a ROCm GPU"):
             int8.int8_linear_train(x, v)
+
+
+def test_linears_too_wide_for_a_row_stay_as_they_are():
+    wide = nn.Linear(32784, 16, device="meta")
+    with pytest.raises(ValueError, match="at most 32768 input features, got 32784"):
+        int8.Int8Linear.from_linear(wide)
+    with pytest.raises(ValueError, match="at most 32768 input features, got 32784"):
+        int8.Int8Linear(32784, 16, device="meta")
+    m = nn.Module()
+    m.blocks = nn.ModuleList([nn.ModuleDict({"wide": wide, "full": nn.Linear(32768, 16, device="meta"),
+                                             "out": nn.Linear(16, 65536, device="meta")})])
+    m, info = int8.convert_model_to_int8(m, keep_bf16_blocks=0, verbose=False)
+    assert info["int8_converted_linears"] == 2 and m.blocks[0]["wide"] is wide
+    assert type(m.blocks[0]["full"]) is type(m.blocks[0]["out"]) is int8.Int8Linear
