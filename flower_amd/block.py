@@ -33,6 +33,7 @@ from types import SimpleNamespace
 
 import torch
 import torch.nn as nn
+from torch.nn.modules import module as nn_module
 
 from . import _lib
 from .attention import CausalSelfAttention
@@ -219,6 +220,19 @@ def _fp8_gated_ok(x: torch.Tensor, ff) -> bool:
 def _hip_rows_ok(*ts: torch.Tensor) -> bool:
     """bf16 GPU tensors whose last dimension the row kernels take (a multiple of 8)."""
     return all(t.is_cuda and t.dtype == torch.bfloat16 for t in ts) and ts[0].shape[-1] % 8 == 0
+
+
+def _bare(*modules: nn.Module) -> bool:
+    """A call of each module runs its class's forward and nothing else: no hooks, no forward of its own but a weight cache's."""
+    if nn_module._global_forward_hooks or nn_module._global_forward_pre_hooks:
+        return False
+    for m in modules:
+        if m._forward_hooks or m._forward_pre_hooks:
+            return False
+        own = m.__dict__.get("forward")                  # a cache that was left leaves the class's, bound
+        if own is not None and not hasattr(own, "of_weight_cache") and getattr(own, "__func__", None) is not type(m).forward:
+            return False
+    return True
 
 
 class RMSNorm(nn.Module):
@@ -490,7 +504,8 @@ class TransformerBlock(nn.Module):
     config's window; RMSNorm norms (``norm_type: rmsnorm``, the 450M configs' choice).
 
     With every Linear an ``Int8Linear`` (``convert_model_to_int8``) and no gradient to take, the norms and the activation are
-    written as the next linear's int8 rows (``_forward_int8``): a call in 8 bits end to end but for the attention."""
+    written as the next linear's int8 rows (``_forward_int8``): a call in 8 bits end to end but for the attention. Modules of the
+    block that have hooks, a ``forward`` of their own or another class run one after the other instead, as with gradients."""
 
     def __init__(self, config) -> None:
         super().__init__()
@@ -502,11 +517,25 @@ class TransformerBlock(nn.Module):
         self.ff = FeedForward(config)
 
     def _int8_ok(self, x: torch.Tensor) -> bool:
-        return (type(self.attn.qkv) is Int8Linear and not torch.is_grad_enabled()
+        attn, ff = self.attn, self.ff
+        if not (type(attn.qkv) is Int8Linear and not torch.is_grad_enabled()
                 and x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 3 and x.numel() > 0
-                and not torch.is_autocast_enabled("cuda") and x.shape[-1] <= 32768 and self.ff.linears()[-1].in_features <= 32768
+                and not torch.is_autocast_enabled("cuda") and x.shape[-1] <= 32768
+                and type(attn) is CausalSelfAttention and type(ff) is FeedForward and type(self.ln1) is type(self.ln2) is RMSNorm):
+            return False
+        passed_by, linears = [attn, ff, self.ln1, self.ln2], [attn.qkv, attn.out]
+        if ff.activation == "gelu":
+            net = list(ff.net._modules.values())
+            if not (type(ff.net) is nn.Sequential and len(net) == 4 and type(net[1]) is nn.GELU and net[1].approximate == "none"
+                    and type(net[2]) is nn.Identity):
+                return False
+            passed_by += [ff.net, *net[1:3]]
+            linears += net[::3]
+        else:
+            linears += ff.linears()
+        return (all(type(m) is Int8Linear for m in linears) and linears[-1].in_features <= 32768
                 and all(w.dtype in (torch.bfloat16, torch.float32) for w in (self.ln1.weight, self.ln2.weight))
-                and all(type(m) is Int8Linear for m in (self.attn.out, *self.ff.linears())))
+                and _bare(*linears, *passed_by) and "qkv_heads" not in attn.__dict__ and "forward_cached" not in attn.__dict__)
 
     def _forward_int8(self, x: torch.Tensor, attend) -> torch.Tensor:
         """The block with int8 linears; attend: from the qkv projection to what ``out`` takes. The norms' outputs stay in fp32 up to

@@ -496,6 +496,7 @@ class fp8_weight_cache:
                 entry = _CachedLayer(mod, mod.forward, self._fingerprint(mod.weight) if self.verify else None)
                 mod.forward = (lambda x, x_amax=None, residual=None, _m=mod, _c=codes:
                                _m.forward_with(x, *_c, x_amax=x_amax, residual=residual))
+                mod.forward.of_weight_cache = True      # not a caller's own forward
                 self.entries.append(entry)
         return self
 
