@@ -68,8 +68,7 @@ class Int8Linear(Fp8Linear):
         if cached is not None:
             return cached
         codes = quantize_weight_cols(self.weight, "rowwise")
-        if getattr(self, "_fp8_cached", None) is not None:       # a cache context is active
-            self._fp8_cached_cols = codes
+        self._keep_cols(codes)
         return codes
 
     def forward_with(self, x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, x_amax=None, residual=None,

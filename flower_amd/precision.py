@@ -370,9 +370,14 @@ class Fp8Linear(nn.Linear):
         if cached is not None:
             return cached
         codes = quantize_weight_cols(self.weight, self.recipe)
-        if getattr(self, "_fp8_cached", None) is not None:       # a cache context is active
-            self._fp8_cached_cols = codes
+        self._keep_cols(codes)
         return codes
+
+    def _keep_cols(self, codes) -> None:
+        """codes for the rest of a cache's context, if one is active. A graph under capture has recorded them, not made them: its
+        replays make their own, and a call outside of it must."""
+        if getattr(self, "_fp8_cached", None) is not None and not torch.cuda.is_current_stream_capturing():
+            self._fp8_cached_cols = codes
 
     def forward_with(self, x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, x_amax=None,
                      residual=None, w8t=None) -> torch.Tensor:
