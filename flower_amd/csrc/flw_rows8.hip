@@ -101,10 +101,10 @@ __device__ __forceinline__ float silu(float x) {
 }
 
 // x Phi(x) = max(x, 0) - |x| Q(|x|), where Q(z) = 1 - Phi(z) = exp(-z^2 / 2) R(z). R is smooth and slow, as 1 / z is: a polynomial of
-// degree 9 in t = 1 / (1 + z / 4), fitted to z <= 14 (relative error 1.4e-8; Q(14) is below fp32). One exponential, one
-// reciprocal with its correction and 9 products, where erff takes a wave of mixed values through both of its ranges. Of normal bf16
-// values a result is off by 6e-8 of itself on average, 7e-7 at most (0.5 x (1 + erf): 2.9e-7, and a third of itself at x = -5, where
-// the sum cancels). -inf gives the limit, 0. [32768, 4096] into e4m3: 119 us, 129 with erff.
+// degree 9 in t = 1 / (1 + z / 4), fitted to z <= 14 (relative error 2.8e-8 with its coefficients in fp32; Q(14) is below fp32). One
+// exponential, one reciprocal with its correction and 9 products, where erff takes a wave of mixed values through both of its
+// ranges. Of normal bf16 values a result is off by 6e-8 of itself on average, 7e-7 at most (0.5 x (1 + erf): 2.9e-7, and a third of
+// itself at x = -5, where the sum cancels). -inf gives the limit, 0. [32768, 4096] into e4m3: 119 us, 129 with erff.
 __device__ __forceinline__ float gelu(float x) {
   const float z = fminf(fabsf(x), 16.0f), d = fmaf(0.25f, z, 1.0f);
   float t = __builtin_amdgcn_rcpf(d), r = 0.033946678042411804f;
