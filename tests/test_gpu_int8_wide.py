@@ -1,4 +1,5 @@
-"""GPU: int8 linears at the ends of what they take: outputs wider than a pass over 8-bit rows, more rows than a column sum.
+"""GPU: int8 linears at the ends of what they take: outputs wider than a pass over 8-bit rows, more rows than a column sum,
+the few-row kernel's largest LDS.
 
 Tolerances as in test_gpu_int8_linear.py: a gradient is off by its bf16 rounding, 2^-8, and the matrix unit's fp32 sums, a thousandth
 of the largest.
@@ -9,7 +10,7 @@ import pytest
 import torch
 
 from flower_amd import int8
-from flower_amd.kernels import int8_linear, quant_rows
+from flower_amd.kernels import int8_linear, int8_scaled_mm, quant_rows
 from oracle.gemm import fp8_linear_backward
 from tests.gpu_util import seeded, to_np
 
@@ -66,3 +67,16 @@ def test_gradients_of_very_many_rows(rows):
     few = [x[some].clone().requires_grad_(), w.detach(), b.detach()]
     assert torch.equal(gx[some], torch.autograd.grad(int8.int8_linear_train(*few), few[0], g[some])[0])
     assert torch.isfinite(gw).all() and gw.any()
+
+
+@pytest.mark.parametrize("M,N,K", [(16, 64, 8960), (15, 100, 9600), (9, 33, 15984), (4, 1283, 32768)])
+def test_few_rows_in_the_most_lds(M, N, K):
+    """Rows that fill the few-row kernel's 150 KB, and those that just do not fit: to the bit, as their float64 sums."""
+    g = torch.Generator().manual_seed(M + N + K)
+    a, b = (torch.randint(-128, 128, (n, K), generator=g).to(torch.int8).cuda() for n in (M, N))
+    sa, sb = (torch.rand(n, generator=g).add(0.5).mul(1e-3).cuda() for n in (M, N))
+    want = (a.double() @ b.double().t()).float().mul_(sa[:, None]).mul_(sb).bfloat16()
+    assert torch.equal(int8_scaled_mm(a, sa, b, sb), want)
+    x = seeded((M, K), 8, torch.bfloat16)
+    codes, scale = quant_rows(x)
+    assert torch.equal(int8_linear(x, b, sb), int8_scaled_mm(codes, scale, b, sb))
