@@ -22,9 +22,14 @@ from .precision import Fp8Linear, fp8_module_filter, quantize_weight_cols
 MAX_IN_FEATURES = 32768
 
 
+def _row_type(t: torch.Tensor | None) -> torch.Tensor | None:
+    """t in a type that the operators take: bfloat16 unless it is that or float32."""
+    return t if t is None or t.dtype in (torch.bfloat16, torch.float32) else t.to(torch.bfloat16)
+
+
 def quantize_weight_int8(weight: torch.Tensor):
     """(codes (N, K) int8, scale (N,) float32) of a weight: one scale an output channel."""
-    return quant_rows(weight.detach())
+    return quant_rows(_row_type(weight.detach()))
 
 
 def int8_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -43,7 +48,8 @@ def _check_width(in_features: int) -> None:
 class Int8Linear(Fp8Linear):
     """``nn.Linear`` in int8 (see the module). Shares the Parameters of the Linear it was built from. The weight is quantised
     on every call unless an ``fp8_weight_cache`` is active. At most 32768 input features. ``forward_codes`` takes the input as
-    codes and scales already, from ``rms_norm_quant`` or another of the passes of ``flower_amd.kernels``."""
+    codes and scales already, from ``rms_norm_quant`` or another of the passes of ``flower_amd.kernels``. The output is bfloat16;
+    inputs and Parameters that are neither bfloat16 nor float32 are cast to it."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None) -> None:
         _check_width(in_features)
@@ -76,14 +82,13 @@ class Int8Linear(Fp8Linear):
         """x_amax and w8t are of the tensorwise recipe: not used."""
         if torch.is_autocast_enabled("cuda"):
             x = x.to(torch.get_autocast_dtype("cuda"))
-        elif x.dtype not in (torch.bfloat16, torch.float32):
-            x = x.to(torch.bfloat16)
+        x = _row_type(x)
         cols = (None, None)
         if (getattr(self, "_fp8_cached", None) is not None and self.backward_fp8 and torch.is_grad_enabled() and x.requires_grad
                 and self.in_features % 16 == 0 and self.out_features % 16 == 0):
             cols = self.weight_col_codes()              # kept for the cache's length; without one the backward makes its own
-        return _lib.native().int8_linear_train(x, self.weight, self.bias, residual, w8, w_scale, *cols, self.backward_fp8,
-                                               _lib.stream_or_none(x))
+        return _lib.native().int8_linear_train(x, _row_type(self.weight), _row_type(self.bias), residual, w8, w_scale, *cols,
+                                               self.backward_fp8, _lib.stream_or_none(x))
 
     def forward(self, x: torch.Tensor, x_amax=None, residual=None) -> torch.Tensor:
         return self.forward_with(x, *self.weight_codes(), residual=residual)
@@ -91,7 +96,7 @@ class Int8Linear(Fp8Linear):
     @torch.no_grad()
     def forward_codes(self, codes: torch.Tensor, scale: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """The output for an input in int8: codes (.., in_features) and scale (..). Forward-only."""
-        return int8_scaled_mm(codes, scale, *self.weight_codes(), bias=self.bias, residual=residual)
+        return int8_scaled_mm(codes, scale, *self.weight_codes(), bias=_row_type(self.bias), residual=residual)
 
 
 def convert_model_to_int8(model: nn.Module, *, keep_bf16_blocks: int = 1, verbose: bool = True):
