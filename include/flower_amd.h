@@ -657,7 +657,7 @@ int flw_rows8_swiglu(const void* gate, const void* up, int dtype, int64_t rows, 
                      int64_t up_row_stride, int code_type, void* codes, int64_t codes_row_stride, float* scale, void* stream);
 
 /* Column sums of bf16 rows x [rows, cols] (a bias's gradient) in fp32, in a fixed order, rounded once to out [cols], fp32 or bf16
- * (out_dtype). Rows of any alignment. workspace: flw_col_sum_workspace_bytes(rows, cols), 16-byte aligned. */
+ * (out_dtype). Rows of any alignment, at most 65535 * 128. workspace: flw_col_sum_workspace_bytes(rows, cols), 16-byte aligned. */
 size_t flw_col_sum_workspace_bytes(int64_t rows, int64_t cols);
 int flw_col_sum(const void* x, int64_t rows, int64_t cols, int64_t x_row_stride, void* out, int out_dtype, void* workspace,
                 size_t workspace_bytes, void* stream);
